@@ -13,7 +13,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libb200moe.so")
 
 OK = 0
-F32, BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 2
 
 STATUS_NAMES = {
     0: "ok", -1: "invalid argument", -2: "unsupported shape", -3: "workspace too small",
@@ -64,6 +64,14 @@ SIGNATURES = {
     "b200moe_ep_combine": (_I, [_P, _P, _P, _I, _I, _I, _P, _P]),
     "b200moe_ep_local_experts": (_I, [_P, _P, _I, _I, _L, _P, _P, _P, _P, _I, _I, _I, _I, _P, _Z, _P, _L, _P]),
     "b200moe_ep_combine_peers": (_I, [_P, _P, _P, _I, _I, _I, _P, _P]),
+    "b200moe_quantize": (_I, [_P, _I, _L, _I, _I, _I, _P, _L, _P, _L, _L, _P]),
+    "b200moe_block_matmul": (_I, [_P, _L, _P, _L, _L, _P, _L, _P, _L, _L, _I, _I, _I, _P, _I, _L, _P, _P]),
+    "b200moe_sort_rows": (_L, [_L, _I, _I, _I]),
+    "b200moe_sort_workspace_bytes": (_L, [_I]),
+    "b200moe_sort_tokens": (_I, [_P, _I, _L, _L, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P, _Z, _P]),
+    "b200moe_permute_rows": (_I, [_P, _L, _L, _I, _L, _I, _P, _P, _P, _I, _L, _P, _L, _I, _P]),
+    "b200moe_unpermute_rows": (_I, [_P, _I, _L, _P, _P, _L, _L, _I, _I, _P, _L, _P]),
+    "b200moe_unpermute_grad": (_I, [_P, _I, _L, _P, _L, _P, _L, _P, _P, _P, _I, _L, _I, _I, _L, _P, _L, _P, _P]),
 }
 
 _lib = None

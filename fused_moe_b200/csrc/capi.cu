@@ -13,6 +13,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "host.cuh"
 #include "kernels.cuh"
 
 using namespace b200moe;
@@ -20,17 +21,6 @@ using namespace b200moe;
 namespace {
 
 thread_local char g_cuda_error[256] = "";
-
-int cuda_fail(cudaError_t e, const char* what) {
-  snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s", what, cudaGetErrorString(e));
-  return B200MOE_ERR_CUDA;
-}
-
-#define CUDA_TRY(expr)                                  \
-  do {                                                  \
-    cudaError_t _e = (expr);                            \
-    if (_e != cudaSuccess) return cuda_fail(_e, #expr); \
-  } while (0)
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -54,8 +44,15 @@ std::mutex g_mutex;
 EncodeTiledFn g_encode = nullptr;
 DeviceInfo g_dev[64];
 
-// Once per process: the driver entry point for tensor-map encoding; once per device: the
-// SM count and the opt-in shared memory sizes of the GEMM kernels.
+}  // namespace
+
+namespace b200moe {
+
+int cuda_fail(cudaError_t e, const char* what) {
+  snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s", what, cudaGetErrorString(e));
+  return B200MOE_ERR_CUDA;
+}
+
 int ensure_device(int* num_sms) {
   int dev = 0;
   CUDA_TRY(cudaGetDevice(&dev));
@@ -82,13 +79,14 @@ int ensure_device(int* num_sms) {
     g_dev[dev].num_sms = prop.multiProcessorCount;
     CUDA_TRY(configure_grouped_gemm());
     CUDA_TRY(configure_stream_gemm());
+    CUDA_TRY(configure_block_matmul());
+    CUDA_TRY(configure_sort_rows());
     g_dev[dev].ready = true;
   }
   *num_sms = g_dev[dev].num_sms;
   return B200MOE_OK;
 }
 
-// Bytes in boxes with 128-byte swizzle.
 int encode_tmap(CUtensorMap* map, const void* base, uint32_t rank, const cuuint64_t* dims, const cuuint64_t* strides,
                 const cuuint32_t* box) {
   const cuuint32_t estr[4] = {1, 1, 1, 1};
@@ -102,13 +100,16 @@ int encode_tmap(CUtensorMap* map, const void* base, uint32_t rank, const cuuint6
   return B200MOE_OK;
 }
 
-// rows x K e4m3 matrix, row pitch `pitch` bytes; box = box_rows x 128 bytes, 128-byte swizzle.
 int make_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint64_t k, uint64_t pitch, uint32_t box_rows) {
   cuuint64_t dims[2] = {k, rows};
   cuuint64_t strides[1] = {pitch};
   cuuint32_t box[2] = {(cuuint32_t)kBlockK, box_rows};
   return encode_tmap(map, base, 2, dims, strides, box);
 }
+
+}  // namespace b200moe
+
+namespace {
 
 // GEMM1 weights [e_local][2*inter][k] seen as planes: plane 2e holds expert e's gate rows, plane
 // 2e+1 its up rows.  One box = the same `box_rows` rows of two consecutive planes (gate rows,

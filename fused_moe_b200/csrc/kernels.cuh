@@ -111,6 +111,10 @@ cudaError_t launch_stream_gemm(int mode, int nt, const StreamParams& p, int max_
 cudaError_t configure_stream_gemm();
 bool stream_gemm_fits(int kblocks, int max_tiles, int num_sms);   // its per-CTA tables hold such a call
 
+// once per device, like the two above: the operators beside the layer
+cudaError_t configure_block_matmul();
+cudaError_t configure_sort_rows();
+
 cudaError_t launch_wait_timeout_selftest(int* status, cudaStream_t stream);
 
 cudaError_t launch_requant(const Workspace& ws, int inter, int num_sms, cudaStream_t stream);

@@ -1,0 +1,399 @@
+"""Operators beside the fused layer, for a user's own tensors: the activations' 8-bit format, the dense product in the experts'
+weight format, and tokens sorted by expert and back.
+
+    codes, scale = quantize(x)                        # what ``run`` takes as hidden_states, hidden_states_scale
+    h = block_matmul(codes, scale, w, w_scale)        # [T, N], w [N, K] with 128x128 block scales like an expert's
+    codes, scale = quantize(h, swiglu=True)           # silu gate between the two products of a feed-forward layer
+
+    ids, weights = route(logits, bias, scaling)       # or any router's choice
+    order = sort_tokens(ids)
+    rows = permute(x, order)                          # differentiable
+    out = unpermute(expert_rows, order, weights)      # differentiable in both
+
+The layer from parts is the sequence route, sort_tokens, permute, quantize, block_matmul per expert, quantize with SwiGLU,
+block_matmul, unpermute.  All results repeat bit for bit (there are no atomics on values), every call is asynchronous on the
+current stream of its tensors' device, can be captured into a CUDA graph and allocates only its results (and the sort, above
+8192 pairs, a scratch tensor) from torch's allocator.  Errors: ``TypeError`` / ``ValueError`` for arguments, ``RuntimeError``
+for tensors that are not on one CUDA device, ``MoEError`` for what the library refuses.
+
+The reference has no counterparts: its only public function is the fused layer (solution/python/kernel.py:642-648).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Dict, Optional, Tuple
+
+import torch
+
+from . import _capi
+from ._capi import MoEError
+from .kernel import BLOCK, E_GLOBAL, _as_bytes
+
+_DTYPE = {torch.float32: _capi.F32, torch.bfloat16: _capi.BF16, torch.float16: _capi.F16}
+
+
+class _on:
+    """The device of a call's tensors, current while the call is made, and its current stream."""
+
+    __slots__ = ("device", "before", "stream")
+
+    def __init__(self, device: torch.device):
+        self.device = device
+
+    def __enter__(self):
+        index = self.device.index
+        self.before = torch.cuda.current_device()
+        if self.before != index:
+            torch.cuda.set_device(index)
+        self.stream = torch.cuda.current_stream(index).cuda_stream
+        return self.stream
+
+    def __exit__(self, *exc):
+        if self.before != self.device.index:
+            torch.cuda.set_device(self.before)
+        return False
+
+
+def _cuda(t: torch.Tensor, what: str) -> torch.device:
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} is on {t.device}: fused_moe_b200 runs on CUDA tensors only (there is no CPU path)")
+    return t.device
+
+
+def _same_device(dev: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{name} is on {t.device}, the other arguments on {dev}")
+
+
+def _no_grad(what: str, *tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
+
+
+def _rows2d(t: torch.Tensor, what: str) -> torch.Tensor:
+    """``t`` with unit inner stride and rows that do not overlap (a copy where it has not)."""
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be 2-D, got shape {tuple(t.shape)}")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Row stride in elements (that of a single row is free: torch may say anything)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _check_out(out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, dev: torch.device) -> None:
+    if out.dtype != dtype or tuple(out.shape) != shape or out.device != dev:
+        raise ValueError(f"out must be {dtype} {list(shape)} on {dev}, got {out.dtype} {list(out.shape)} on {out.device}")
+    if (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1]):
+        raise ValueError("out must have unit inner stride and rows that do not overlap")
+    if out.requires_grad:
+        raise RuntimeError("out must not require a gradient")
+
+
+# ---- quantisation ----
+
+def quantize(x: torch.Tensor, *, swiglu: bool = False, scale_layout: str = "kt") -> Tuple[torch.Tensor, torch.Tensor]:
+    """Activations [T, K] (fp32, bf16 or fp16) as (e4m3 codes [T, K], fp32 scales of each 1x128 block).
+
+    ``scale = max(max|x|, 1e-12) / 448`` per block, ``code = e4m3(x / scale)``, the quotient rounded to fp32 first: bit for bit
+    ``synth.quant_rows_1x128``.  ``scale_layout`` "kt" gives the scales as [ceil(K/128), T], the layer's layout, "tk" as
+    [T, ceil(K/128)].  With ``swiglu`` the input is [T, 2K] and what is quantised is ``x[:, :K] * silu(x[:, K:])`` in fp32.
+    A block that holds an infinity or a NaN gets it as its scale, and codes as the quotient says.  Any K; not differentiable.
+    """
+    dev = _cuda(x, "x")
+    dt = _DTYPE.get(x.dtype)
+    if dt is None:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    if scale_layout not in ("kt", "tk"):
+        raise ValueError(f"scale_layout must be 'kt' or 'tk', got {scale_layout!r}")
+    _no_grad("quantize", x)
+    x = _rows2d(x, "x")
+    rows, cols = x.shape
+    if swiglu:
+        if cols % 2:
+            raise ValueError(f"swiglu needs an even number of columns (gate half, up half), got {cols}")
+        cols //= 2
+    blocks = -(-cols // BLOCK)
+    codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=dev)
+    kt = scale_layout == "kt"
+    scale = torch.empty((blocks, rows) if kt else (rows, blocks), dtype=torch.float32, device=dev)
+    if rows == 0 or cols == 0:
+        return codes, scale
+    with _on(dev) as stream:
+        rc = _capi.lib().b200moe_quantize(x.data_ptr(), dt, _pitch(x), rows, cols, int(swiglu), codes.data_ptr(), cols,
+                                          scale.data_ptr(), 1 if kt else blocks, rows if kt else 1, stream)
+    _capi.check(rc, "b200moe_quantize")
+    return codes, scale
+
+
+# ---- block-scaled product ----
+
+class _Status:
+    """Pinned words of one device where a kernel that gave up on a bounded wait leaves its code."""
+
+    def __init__(self):
+        self.words = torch.zeros(4, dtype=torch.int32).pin_memory()
+        self.ptr = self.words.data_ptr()
+        self.view = (C.c_int32 * 4).from_address(self.ptr)
+
+    def raise_if_failed(self):
+        if self.view[0]:
+            code, where = self.view[0], self.view[1]
+            self.view[0] = 0
+            raise MoEError(code, "device status of an earlier b200moe_block_matmul on this device", f"detail={where}")
+
+
+_status: Dict[int, _Status] = {}
+
+
+def _block_scale_strides(scale: torch.Tensor, rows: int, blocks: int, layout: str, what: str) -> Tuple[int, int]:
+    """(stride over rows, stride over K blocks) of a scale tensor, in elements."""
+    want = (blocks, rows) if layout == "kt" else (rows, blocks)
+    if scale.dtype != torch.float32:
+        raise TypeError(f"{what} must be float32, got {scale.dtype}")
+    if tuple(scale.shape) != want:
+        raise ValueError(f"{what} has shape {tuple(scale.shape)}, expected {want} for scale_layout {layout!r}")
+    s0, s1 = scale.stride()
+    return (s1, s0) if layout == "kt" else (s0, s1)
+
+
+def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *, scale_layout: str = "kt",
+                 out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``a @ b.T`` of e4m3 matrices with block scales, accumulated in fp32: [M, N] in ``out_dtype`` (bf16, fp16, fp32).
+
+    a [M, K] e4m3 (or its uint8 bits) with a_scale fp32 per 1x128, [ceil(K/128), M] (``scale_layout`` "kt") or
+    [M, ceil(K/128)] ("tk"); b [N, K] e4m3 with b_scale fp32 [ceil(N/128), ceil(K/128)], the layout of an expert's weights.
+    K must be a multiple of 16, M and N may be any.  Rows of ``a`` whose pitch is not a multiple of 16 bytes are copied; ``b``
+    must have unit inner stride and such a pitch.  Scales may have any strides.  ``out`` writes into a tensor of the caller's
+    (which must not overlap the inputs).  Not differentiable: the operands are codes.
+    """
+    dev = _cuda(a, "a")
+    _same_device(dev, a_scale=a_scale, b=b, b_scale=b_scale)
+    _no_grad("block_matmul", a_scale, b_scale)
+    a, b = _rows2d(_as_bytes(a, "a"), "a"), _as_bytes(b, "b")
+    if b.dim() != 2 or b.shape[1] != a.shape[1]:
+        raise ValueError(f"b must be [N, {a.shape[1]}], got {tuple(b.shape)}")
+    (M, K), N = a.shape, b.shape[0]
+    if K == 0 or K % 16:
+        raise ValueError(f"K must be a positive multiple of 16, got {K}")
+    if scale_layout not in ("kt", "tk"):
+        raise ValueError(f"scale_layout must be 'kt' or 'tk', got {scale_layout!r}")
+    blocks = -(-K // BLOCK)
+    as_m, as_kb = _block_scale_strides(a_scale, M, blocks, scale_layout, "a_scale")
+    bs_n, bs_kb = _block_scale_strides(b_scale, -(-N // BLOCK), blocks, "tk", "b_scale")
+    if b.stride(1) != 1 or (N > 1 and (b.stride(0) < K or b.stride(0) % 16)) or b.data_ptr() % 16:
+        raise ValueError("b must have unit inner stride and rows on 16-byte boundaries")
+    if _pitch(a) % 16 or a.data_ptr() % 16:
+        a = a.contiguous() if a.data_ptr() % 16 == 0 and not a.is_contiguous() else a.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        dt = _DTYPE.get(out_dtype)
+        if dt is None:
+            raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    else:
+        dt = _DTYPE.get(out.dtype)
+        if dt is None:
+            raise TypeError(f"out must be float32, bfloat16 or float16, got {out.dtype}")
+        _check_out(out, (M, N), out.dtype, dev)
+    if M == 0 or N == 0:
+        return out
+    st = _status.get(dev.index)
+    if st is None and not torch.cuda.is_current_stream_capturing():   # (pinned memory cannot be had during a capture)
+        st = _status[dev.index] = _Status()
+    if st is not None:
+        st.raise_if_failed()
+    with _on(dev) as stream:
+        rc = _capi.lib().b200moe_block_matmul(a.data_ptr(), _pitch(a), a_scale.data_ptr(), as_m, as_kb, b.data_ptr(), _pitch(b),
+                                              b_scale.data_ptr(), bs_n, bs_kb, M, N, K, out.data_ptr(), dt, _pitch(out),
+                                              None if st is None else st.ptr, stream)
+    _capi.check(rc, "b200moe_block_matmul")
+    return out
+
+
+# ---- tokens sorted by expert and back ----
+
+class TokenOrder:
+    """What ``sort_tokens`` found; int32 tensors on the ids' device.
+
+    offsets [e_local + 1]  first row of each local expert, the last: rows in use
+    counts  [e_local]      pairs of each local expert
+    pos     [T, top_k]     row of each (token, k), -1 where the expert is not local
+    pair    [rows]         token * top_k + k of each row, -1 in padding and behind the last expert
+    """
+
+    __slots__ = ("offsets", "counts", "pos", "pair", "tokens", "top_k", "rows", "e_local", "local_expert_offset", "align")
+
+    def __init__(self, offsets, counts, pos, pair, e_local, local_expert_offset, align):
+        self.offsets, self.counts, self.pos, self.pair = offsets, counts, pos, pair
+        self.tokens, self.top_k = pos.shape
+        self.rows = pair.shape[0]
+        self.e_local, self.local_expert_offset, self.align = e_local, local_expert_offset, align
+
+
+def sort_tokens(topk_ids: torch.Tensor, e_local: int = E_GLOBAL, local_expert_offset: int = 0, *, align: int = 1) -> TokenOrder:
+    """Stable sort of the pairs (token, k) by expert; ids int32 or int64 [T, top_k], top_k at most 32.
+
+    Experts [local_expert_offset, local_expert_offset + e_local) are local (at most 1024); pairs of others get no row, and an
+    expert that a token names twice gets two.  Each expert's rows start on a multiple of ``align`` (128: a matrix tile).  The
+    order has ``T * top_k`` rows and, with ``align``, room for the padding: how many are in use stays on the device.
+    """
+    dev = _cuda(topk_ids, "topk_ids")
+    if topk_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
+    ids = _rows2d(topk_ids, "topk_ids")
+    tokens, top_k = ids.shape
+    e_local, off, align = int(e_local), int(local_expert_offset), int(align)
+    if not 1 <= top_k <= 32:
+        raise ValueError(f"topk_ids must have 1 to 32 columns, got {top_k}")
+    if not 1 <= e_local <= 1024:
+        raise ValueError(f"e_local must be 1 to 1024, got {e_local}")
+    if not 0 <= off < 2 ** 30:
+        raise ValueError(f"local_expert_offset must not be negative, got {off}")
+    if not 1 <= align <= 65536:
+        raise ValueError(f"align must be 1 to 65536, got {align}")
+    pairs = tokens * top_k
+    rows = -(-(pairs + (align - 1) * min(pairs, e_local)) // align) * align
+    if rows >= 2 ** 31:
+        raise ValueError(f"{rows} sorted rows: int32 tables name at most {2 ** 31 - 1}")
+    # one allocation, the four tables each at a multiple of 16 bytes
+    pos_at = (2 * e_local + 1 + 3) // 4 * 4
+    pair_at = pos_at + (pairs + 3) // 4 * 4
+    table = torch.empty(pair_at + rows, dtype=torch.int32, device=dev)
+    offsets, counts = table[:e_local + 1], table[e_local + 1:2 * e_local + 1]
+    pos, pair = table[pos_at:pos_at + pairs].view(tokens, top_k), table[pair_at:]
+    with _on(dev) as stream:
+        lib = _capi.lib()
+        ws, ws_bytes, ws_ptr = None, 0, None
+        if pairs > 8192:
+            ws_bytes = lib.b200moe_sort_workspace_bytes(e_local)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            ws_ptr = ws.data_ptr()
+        rc = lib.b200moe_sort_tokens(ids.data_ptr(), ids.element_size() * 8, _pitch(ids), tokens, top_k, e_local, off, align,
+                                     counts.data_ptr(), offsets.data_ptr(), pos.data_ptr(), pair.data_ptr(), rows,
+                                     ws_ptr, ws_bytes, stream)
+    _capi.check(rc, "b200moe_sort_tokens")
+    return TokenOrder(offsets, counts, pos, pair, e_local, off, align)
+
+
+def _permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor]) -> torch.Tensor:
+    dev, size, H = x.device, x.element_size(), x.shape[1]
+    x = _rows2d(x, "x")
+    y = torch.empty((order.rows, H), dtype=x.dtype, device=dev) if out is None else out
+    with _on(dev) as stream:
+        rc = _capi.lib().b200moe_permute_rows(x.data_ptr(), _pitch(x) * size, H * size, size, order.tokens, order.top_k,
+                                              order.pos.data_ptr(), order.pair.data_ptr(), order.offsets.data_ptr(),
+                                              order.e_local, order.rows, y.data_ptr(), _pitch(y) * size, int(out is None), stream)
+    _capi.check(rc, "b200moe_permute_rows")
+    return y
+
+
+def _unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tensor], out: Optional[torch.Tensor]) -> torch.Tensor:
+    dev, H = y.device, y.shape[1]
+    y = _rows2d(y, "y")
+    w = None if weights is None else _rows2d(weights, "weights")
+    res = torch.empty((order.tokens, H), dtype=y.dtype, device=dev) if out is None else out
+    with _on(dev) as stream:
+        rc = _capi.lib().b200moe_unpermute_rows(y.data_ptr(), _DTYPE[y.dtype], _pitch(y), order.pos.data_ptr(),
+                                                None if w is None else w.data_ptr(), 0 if w is None else _pitch(w),
+                                                order.tokens, order.top_k, H, res.data_ptr(), _pitch(res), stream)
+    _capi.check(rc, "b200moe_unpermute_rows")
+    return res
+
+
+class _Permute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, order):
+        ctx.order = order
+        return _permute(x, order, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return _unpermute(dy, ctx.order, None, None), None
+
+
+class _Unpermute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, order, weights):
+        ctx.order = order
+        ctx.save_for_backward(y if weights is not None and weights.requires_grad else None, weights)
+        ctx.y_like = (y.shape, y.dtype)
+        return _unpermute(y, order, weights, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        order, (y, weights) = ctx.order, ctx.saved_tensors
+        (rows, H), dtype = ctx.y_like
+        dev = dout.device
+        dout = _rows2d(dout, "grad")
+        dy = torch.empty((rows, H), dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = torch.empty((order.tokens, order.top_k), dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
+        y = None if dw is None else _rows2d(y, "y")
+        w = None if weights is None else _rows2d(weights, "weights")
+        with _on(dev) as stream:
+            rc = _capi.lib().b200moe_unpermute_grad(
+                dout.data_ptr(), _DTYPE[dtype], _pitch(dout), None if y is None else y.data_ptr(), 0 if y is None else _pitch(y),
+                None if w is None else w.data_ptr(), 0 if w is None else _pitch(w), order.pos.data_ptr(), order.pair.data_ptr(),
+                order.offsets.data_ptr(), order.e_local, order.tokens, order.top_k, H, rows,
+                None if dy is None else dy.data_ptr(), H, None if dw is None else dw.data_ptr(), stream)
+        _capi.check(rc, "b200moe_unpermute_grad")
+        return dy, None, dw
+
+
+def permute(x: torch.Tensor, order: TokenOrder, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rows of x [T, H] in the sorted order, [order.rows, H]: ``y[pos[t, k]] = x[t]``, zeros in padding rows.
+
+    Any type of 1, 2 or 4 bytes an element (e4m3 codes and their "tk" scales among them).  Rows behind the last expert are
+    zero too, except in an ``out`` of the caller's, where they stay as they were.  Differentiable for fp32, bf16 and fp16 x
+    (without ``out``): ``dx[t]`` is the sum of dy over the token's rows, in fp32, rounded once.
+    """
+    dev = _cuda(x, "x")
+    _same_device(dev, order=order.pos)
+    if x.dim() != 2 or x.shape[0] != order.tokens:
+        raise ValueError(f"x must be [{order.tokens}, H], got {tuple(x.shape)}")
+    if x.element_size() not in (1, 2, 4) or x.is_complex():
+        raise TypeError(f"x must have elements of 1, 2 or 4 bytes, got {x.dtype}")
+    if x.requires_grad and torch.is_grad_enabled():
+        if out is not None:
+            raise RuntimeError("permute with out= has no gradient: detach x or leave out away")
+        if x.dtype not in _DTYPE:
+            raise TypeError(f"permute has no gradient for {x.dtype}")
+        return _Permute.apply(x, order)
+    if out is not None:
+        _check_out(out, (order.rows, x.shape[1]), x.dtype, dev)
+    return _permute(x, order, out)
+
+
+def unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tensor] = None, *,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Sums of each token's rows: ``out[t] = sum_k weights[t, k] * y[pos[t, k]]``, k ascending, fp32, rounded once to y's type.
+
+    y [order.rows, H] fp32, bf16 or fp16; weights fp32 [T, top_k], or None for ones.  Choices that are not local add nothing (a
+    token without any is zero) whatever their weight.  Differentiable in y and weights (without ``out``): rows of dy that no
+    pair takes are zero, dw is 0 where the expert is not local.
+    """
+    dev = _cuda(y, "y")
+    _same_device(dev, order=order.pos, weights=weights)
+    if y.dtype not in _DTYPE:
+        raise TypeError(f"y must be float32, bfloat16 or float16, got {y.dtype}")
+    if y.dim() != 2 or y.shape[0] != order.rows:
+        raise ValueError(f"y must be [{order.rows}, H], got {tuple(y.shape)}")
+    if weights is not None:
+        if weights.dtype != torch.float32:
+            raise TypeError(f"weights must be float32, got {weights.dtype}")
+        if tuple(weights.shape) != (order.tokens, order.top_k):
+            raise ValueError(f"weights must be [{order.tokens}, {order.top_k}], got {tuple(weights.shape)}")
+    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
+        if out is not None:
+            raise RuntimeError("unpermute with out= has no gradient: detach its inputs or leave out away")
+        return _Unpermute.apply(y, order, weights)
+    if out is not None:
+        _check_out(out, (order.tokens, y.shape[1]), y.dtype, dev)
+    return _unpermute(y, order, weights, out)

@@ -53,7 +53,8 @@ typedef enum b200moe_status {
 
 typedef enum b200moe_dtype {
   B200MOE_F32 = 0,
-  B200MOE_BF16 = 1
+  B200MOE_BF16 = 1,
+  B200MOE_F16 = 2      /* operators beside the layer only; logits and bias are fp32 or bf16 */
 } b200moe_dtype;
 
 /* Byte offsets of the intermediates inside a workspace, for tests and tools.
@@ -266,6 +267,77 @@ B200MOE_API int b200moe_ep_local_experts(const void* const* send_base, const int
 B200MOE_API int b200moe_ep_combine_peers(const void* const* partial_bf16, const int32_t* row_start,
                         const int32_t* send_slot, int T, int hidden, int world,
                         void* out_bf16, void* stream);
+
+/* ---- operators beside the layer (no counterparts in the reference, which has the fused layer only): the layer's
+ * activation format, the dense product in the experts' weight format, and tokens sorted by expert and back for experts that
+ * the fused layer does not know.  Nothing here reads a workspace of the layer; all results repeat bit for bit. ---- */
+
+/* Activations to e4m3 with one scale per 1x128 block, what b200moe_run and b200moe_block_matmul take:
+ *   scale[t,b] = max(max |x[t,k]| over block b, 1e-12) / 448, codes[t,k] = e4m3(fp32(x[t,k] / scale[t,b]))
+ * (round to nearest even).  A block with an infinity or a NaN gets that scale, and codes as the quotient says.
+ *  x        [rows, cols] of `dtype` (fp32, bf16, fp16), `row_stride` elements; swiglu != 0: [rows, 2 cols], and
+ *           x[t,k] = in[t,k] * silu(in[t,cols+k]) in fp32 (the layer's order: gate half first, silu on the second)
+ *  codes    [rows, cols] bytes, `codes_row_stride` bytes
+ *  scale    fp32, element (t, b) at scale[t*scale_stride_t + b*scale_stride_kb], ceil(cols/128) blocks a row.
+ * Any cols; the last block may be short. */
+B200MOE_API int b200moe_quantize(const void* x, int dtype, int64_t row_stride, int rows, int cols, int swiglu,
+                     uint8_t* codes, int64_t codes_row_stride,
+                     float* scale, int64_t scale_stride_t, int64_t scale_stride_kb, void* stream);
+
+/* out[m,n] = sum_b a_scale[m,b] * b_scale[n/128,b] * sum_{k in block b} a[m,k] * b[n,k], accumulated in fp32, rounded once.
+ *  a        e4m3 [M, K], b e4m3 [N, K] (the experts' weight layout); row strides in bytes, multiples of 16; bases 16-byte aligned
+ *  a_scale  fp32, element (m, b) at a_scale[m*a_scale_stride_m + b*a_scale_stride_kb]
+ *  b_scale  fp32, element (n/128, b) at b_scale[(n/128)*b_scale_stride_n + b*b_scale_stride_kb]
+ *  out      [M, N] of `out_dtype` (fp32, bf16, fp16), `out_row_stride` elements
+ *  status   optional device-accessible int32[2] (e.g. host-mapped), written only when a bounded device-side wait gave up:
+ *           [0] = B200MOE_ERR_DEVICE_TIMEOUT, [1] = where.
+ * K a multiple of 16 (the last block may be short); M, N any. */
+B200MOE_API int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride,
+                         const float* a_scale, int64_t a_scale_stride_m, int64_t a_scale_stride_kb,
+                         const uint8_t* b, int64_t b_row_stride,
+                         const float* b_scale, int64_t b_scale_stride_n, int64_t b_scale_stride_kb,
+                         int M, int N, int K, void* out, int out_dtype, int64_t out_row_stride,
+                         int32_t* status, void* stream);
+
+/* Rows of the sorted order of tokens x top_k pairs: every pair, and room to start each expert on a multiple of `align`.
+ * Negative: a status (bad argument). */
+B200MOE_API int64_t b200moe_sort_rows(int64_t tokens, int top_k, int e_local, int align);
+
+/* Bytes of workspace that b200moe_sort_tokens needs for any number of tokens.  Negative: a status. */
+B200MOE_API int64_t b200moe_sort_workspace_bytes(int e_local);
+
+/* Stable sort of the pairs (t, k) by expert.  ids of `ids_bits` 32 or 64, `ids_row_stride` elements; an id outside
+ * [local_expert_offset, local_expert_offset + e_local) is not local and gets no row; an expert that a token names twice gets
+ * two rows.  e_local 1..1024, top_k 1..32, align 1..65536.
+ *  counts   int32[e_local]      pairs of each local expert
+ *  offsets  int32[e_local + 1]  first row of each (multiples of align); the last is the number of rows in use
+ *  pos      int32[tokens][top_k] row of each pair, -1: not local
+ *  pair     int32[rows]         t*top_k + k of each row, -1: padding, or behind the last segment
+ *  rows     length of `pair`, at least b200moe_sort_rows(...)
+ *  workspace may be NULL up to 8192 pairs. */
+B200MOE_API int b200moe_sort_tokens(const void* topk_ids, int ids_bits, int64_t ids_row_stride, int64_t tokens, int top_k,
+                        int e_local, int local_expert_offset, int align,
+                        int32_t* counts, int32_t* offsets, int32_t* pos, int32_t* pair, int64_t rows,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* y[pos[t,k]] = x[t]; padding rows become zero, rows behind the last segment too if zero_tail, else they are left as they were.
+ * Rows are `row_bytes` of elements of `elem_bytes` 1, 2 or 4; x_row_bytes and y_row_bytes are the row pitches. */
+B200MOE_API int b200moe_permute_rows(const void* x, int64_t x_row_bytes, int64_t row_bytes, int elem_bytes, int64_t tokens,
+                         int top_k, const int32_t* pos, const int32_t* pair, const int32_t* offsets, int e_local, int64_t rows,
+                         void* y, int64_t y_row_bytes, int zero_tail, void* stream);
+
+/* out[t] = sum over k with pos[t,k] >= 0 of weights[t,k] * y[pos[t,k]], k ascending, in fp32, rounded once to `dtype`
+ * (fp32, bf16, fp16); weights NULL: ones (then it is the gradient of b200moe_permute_rows).  Strides in elements. */
+B200MOE_API int b200moe_unpermute_rows(const void* y, int dtype, int64_t y_row_stride, const int32_t* pos,
+                           const float* weights, int64_t w_row_stride, int64_t tokens, int top_k, int hidden,
+                           void* out, int64_t out_row_stride, void* stream);
+
+/* Gradient of b200moe_unpermute_rows: dy[pos[t,k]] = weights[t,k] * dout[t] (all other rows of dy become zero) and
+ * dw[t,k] = <dout[t], y[pos[t,k]]> in fp32, 0 where pos is -1.  dy or dw may be NULL (not wanted; y is read for dw only). */
+B200MOE_API int b200moe_unpermute_grad(const void* dout, int dtype, int64_t dout_row_stride, const void* y, int64_t y_row_stride,
+                           const float* weights, int64_t w_row_stride, const int32_t* pos, const int32_t* pair,
+                           const int32_t* offsets, int e_local, int64_t tokens, int top_k, int hidden, int64_t rows,
+                           void* dy, int64_t dy_row_stride, float* dw /* [tokens][top_k] */, void* stream);
 
 #ifdef __cplusplus
 }
