@@ -67,7 +67,7 @@ SIGNATURES = {
     "b200moe_quantize": (_I, [_P, _I, _L, _I, _I, _I, _P, _L, _P, _L, _L, _P]),
     "b200moe_block_matmul": (_I, [_P, _L, _P, _L, _L, _P, _L, _P, _L, _L, _I, _I, _I, _P, _I, _L, _P, _P]),
     "b200moe_sort_rows": (_L, [_L, _I, _I, _I]),
-    "b200moe_sort_workspace_bytes": (_L, [_I]),
+    "b200moe_sort_workspace_bytes": (_L, [_L, _I, _I]),
     "b200moe_sort_tokens": (_I, [_P, _I, _L, _L, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P, _Z, _P]),
     "b200moe_permute_rows": (_I, [_P, _L, _L, _I, _L, _I, _P, _P, _P, _I, _L, _P, _L, _I, _P]),
     "b200moe_unpermute_rows": (_I, [_P, _I, _L, _P, _P, _L, _L, _I, _I, _P, _L, _P]),

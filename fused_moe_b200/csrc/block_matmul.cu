@@ -43,18 +43,6 @@ struct MatmulParams {
   int* status;                                   // device-accessible int32[2], or null
 };
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t smem_addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
-  return r;
-}
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, float a, float b, float c, float d) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
@@ -335,19 +323,7 @@ extern "C" int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride, cons
   p.split = 1;
   while (p.split < kMaxSplit && m_tiles * n_tiles * p.split * 2 <= 2 * num_sms && p.kblocks >= 4 * p.split) p.split *= 2;
 
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(m_tiles * n_tiles * p.split));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = chained_launch_enabled() ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)p.split;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.split > 1 ? 2 : 1;
-  CUDA_TRY(cudaLaunchKernelEx(&cfg, block_matmul_kernel, p));
+  CUDA_TRY(launch_chained_cluster(block_matmul_kernel, dim3((unsigned)(m_tiles * n_tiles * p.split)), dim3(kThreads), kSmemBytes,
+                                  reinterpret_cast<cudaStream_t>(stream), p.split, p));
   return B200MOE_OK;
 }

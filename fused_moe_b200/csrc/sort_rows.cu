@@ -19,64 +19,69 @@ namespace {
 
 constexpr int kMaxSortExperts = 1024;
 constexpr int kMaxSortTopK = 32;                 // a token's positions are held by the lanes of a warp
-constexpr int kSortThreads = 1024;
-constexpr int kSortChunk = 4096;                 // pairs of a CTA, until there is one for each SM
-constexpr int kSortOneBlock = 8192;              // up to so many pairs one CTA sorts alone, in one launch
+constexpr int kSortWarps = 16;
+constexpr int kSortThreads = 32 * kSortWarps;
+constexpr int kSortCluster = 8;                  // CTAs that one launch sorts with
+constexpr int kSortRounds = 4, kSortManyRounds = 16;   // pairs of a thread
 
 struct SortParams {
   const void* ids;
   long long ids_stride;
-  long long pairs;
-  int top_k;
+  int pairs, top_k;
+  int contiguous;                                // ids_stride == top_k
   int wide;                                      // int64 ids
+  int vec_pair;                                  // what lies behind the last segment starts on 16 bytes of `pair`
   int local_off, e_local, align;
-  long long rows;                                // length of `pair`
+  int rows;                                      // length of `pair`
   int* counts;                                   // [e_local]
   int* offsets;                                  // [e_local + 1]
   int* pos;                                      // [pairs]
   int* pair;                                     // [rows]
-  int* chunk_counts;                             // [chunks][e_local]
-  long long chunk;                               // pairs of a CTA
+  int* chunk_counts;                             // [chunks][e_local] of the kernel before; null: the chunks are one cluster
   int chunks;
 };
 
-__device__ __forceinline__ int local_expert(const SortParams& p, long long i) {
-  const long long t = i / p.top_k;
-  const long long at = t * p.ids_stride + (i - t * p.top_k);
+__device__ __forceinline__ int local_expert(const SortParams& p, int i) {
+  long long at = i;
+  if (!p.contiguous) {
+    const int t = i / p.top_k;
+    at = t * p.ids_stride + (i - t * p.top_k);
+  }
   const long long id = p.wide ? reinterpret_cast<const long long*>(p.ids)[at] : (long long)reinterpret_cast<const int*>(p.ids)[at];
   return id >= p.local_off && id < (long long)p.local_off + p.e_local ? (int)(id - p.local_off) : -1;
 }
 
-// Pairs [begin, end) of one warp, counted per expert into its own row of shared counters.
-__device__ __forceinline__ void count_range(const SortParams& p, long long begin, long long end, int lane, int* cnt) {
-  for (long long i = begin + lane; i < end; i += 32) {
-    const int e = local_expert(p, i);
-    if (e >= 0) atomicAdd(cnt + e, 1);
+// Expert of each of a thread's R pairs (-1: not local, or past the end): warp w of chunk c has pairs
+// [(c * kSortWarps + w) * 32 R, + 32 R), round r its 32 from 32 r on.  All loads are in flight together.
+template <int R>
+__device__ __forceinline__ long long load_experts(const SortParams& p, int (&e)[R]) {
+  const long long first = ((long long)blockIdx.x * kSortWarps + (threadIdx.x >> 5)) * (32 * R) + (threadIdx.x & 31);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const long long i = first + r * 32;
+    e[r] = i < p.pairs ? local_expert(p, (int)i) : -1;
   }
+  return first;
 }
 
-__device__ __forceinline__ void warp_range(const SortParams& p, int warp, int warps, long long* begin, long long* end) {
-  const long long first = (long long)blockIdx.x * p.chunk, last = min(first + p.chunk, p.pairs);
-  const long long share = ((last - first + warps - 1) / warps + 31) / 32 * 32;
-  *begin = min(first + warp * share, last);
-  *end = min(*begin + share, last);
-}
-
+template <int R>
 __global__ void __launch_bounds__(kSortThreads)
 sort_count_kernel(const __grid_constant__ SortParams p) {
   extern __shared__ int s_cnt[];                 // [e_local]
-  for (int e = threadIdx.x; e < p.e_local; e += blockDim.x) s_cnt[e] = 0;
-  __syncthreads();
+  for (int e = threadIdx.x; e < p.e_local; e += kSortThreads) s_cnt[e] = 0;
   chain_wait();
   chain_release();
-  long long begin, end;
-  warp_range(p, threadIdx.x >> 5, blockDim.x >> 5, &begin, &end);
-  count_range(p, begin, end, threadIdx.x & 31, s_cnt);
+  int e[R];
+  load_experts<R>(p, e);
   __syncthreads();
-  for (int e = threadIdx.x; e < p.e_local; e += blockDim.x) p.chunk_counts[(size_t)blockIdx.x * p.e_local + e] = s_cnt[e];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (e[r] >= 0) atomicAdd(s_cnt + e[r], 1);
+  __syncthreads();
+  for (int x = threadIdx.x; x < p.e_local; x += kSortThreads) p.chunk_counts[(size_t)blockIdx.x * p.e_local + x] = s_cnt[x];
 }
 
-// Exclusive sum over the CTA's 1024 threads.
+// Exclusive sum over the CTA's threads.
 __device__ __forceinline__ int block_exclusive_sum(int v, int* s_warp, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int sum = v;
@@ -87,125 +92,188 @@ __device__ __forceinline__ int block_exclusive_sum(int v, int* s_warp, int* tota
   }
   if (lane == 31) s_warp[warp] = sum;
   __syncthreads();
-  if (warp == 0) {
-    int w = s_warp[lane];
+  int before = 0, all = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += up;
-    }
-    s_warp[lane] = w;
+  for (int w = 0; w < kSortWarps; ++w) {
+    const int x = s_warp[w];
+    before += w < warp ? x : 0;
+    all += x;
   }
-  __syncthreads();
-  *total = s_warp[31];
-  return sum - v + (warp > 0 ? s_warp[warp - 1] : 0);
+  *total = all;
+  return sum - v + before;
 }
 
-// Places the pairs of a CTA's chunk.  Each warp owns a run of the chunk and a row of counters: counted once, turned into
-// first rows by a sum over the warps, then walked again, 32 pairs at a time, a pair's place among its warp's by a match of the
-// expert.  A call of one chunk needs no kernel before it.
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Places the pairs of a CTA's chunk.  Each warp owns a run of the chunk and a row of counters; a pair's place among its warp's
+// pairs of the same expert is the counter plus its rank in a match of the expert over the warp, a warp's first place the sum over
+// the warps before it.  What the other chunks hold comes out of their shared memory (the chunks are one cluster: one launch),
+// or out of the kernel before.  What this takes is latency: no loop over anything but rounds, warps and chunks.
+template <int R>
 __global__ void __launch_bounds__(kSortThreads)
-sort_place_kernel(const __grid_constant__ SortParams p, int warps) {
-  extern __shared__ int smem[];
-  int* s_next = smem;                            // [warps][e_local]
-  int* s_total = s_next + warps * p.e_local;     // [e_local] pairs of all chunks
-  int* s_before = s_total + p.e_local;           // [e_local] pairs of the chunks before this one
-  int* s_first = s_before + p.e_local;           // [e_local + 1]
-  int* s_warp = s_first + p.e_local + 1;         // [32]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = p.e_local;
-  for (int i = threadIdx.x; i < (warps + 2) * E; i += blockDim.x) smem[i] = 0;
-  __syncthreads();
+sort_place_kernel(const __grid_constant__ SortParams p) {
+  extern __shared__ __align__(16) int smem[];
+  const int E = p.e_local;
+  int* s_cnt = smem;                             // [kSortWarps][E]
+  int* s_total = s_cnt + kSortWarps * E;         // [E] pairs of all chunks
+  int* s_before = s_total + E;                   // [E] pairs of the chunks before this one
+  int* s_chunk = s_before + E;                   // [E] pairs of this chunk
+  int* s_first = s_chunk + E;                    // [E + 1]
+  __shared__ int s_warp[kSortWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < (kSortWarps + 2) * E; i += kSortThreads) smem[i] = 0;
   chain_wait();
   chain_release();
-  long long begin = 0, end = 0;
-  if (warp < warps) {
-    warp_range(p, warp, warps, &begin, &end);
-    count_range(p, begin, end, lane, s_next + warp * E);
+  int e[R], rank[R];
+  const long long first_pair = load_experts<R>(p, e);
+  __syncthreads();
+  int* mine = s_cnt + warp * E;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const unsigned same = __match_any_sync(0xffffffffu, e[r]);
+    const int before = e[r] >= 0 ? mine[e[r]] : 0;
+    rank[r] = before + __popc(same & ((1u << lane) - 1u));
+    __syncwarp();
+    if (e[r] >= 0 && lane == 31 - __clz(same)) mine[e[r]] = rank[r] + 1;
+    __syncwarp();
   }
-  if (p.chunks > 1) {                            // all threads: parts of the columns of the chunk counts
-    const int parts = blockDim.x / E > 0 ? blockDim.x / E : 1;
-    const int per = (p.chunks + parts - 1) / parts;
-    for (int i = threadIdx.x; i < parts * E; i += blockDim.x) {
-      const int e = i % E, c0 = i / E * per, c1 = min(c0 + per, p.chunks);
+  __syncthreads();
+  for (int x = threadIdx.x; x < E; x += kSortThreads) {
+    int n[kSortWarps], sum = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) n[w] = s_cnt[w * E + x];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+      s_cnt[w * E + x] = sum;
+      sum += n[w];
+    }
+    s_chunk[x] = sum;
+  }
+  const bool cluster = p.chunks > 1 && !p.chunk_counts;
+  if (cluster) {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    for (int x = threadIdx.x; x < E; x += kSortThreads) {
+      const uint32_t addr = smem_u32(s_chunk + x);
+      int n[kSortCluster];
+#pragma unroll
+      for (int c = 0; c < kSortCluster; ++c) n[c] = c < p.chunks ? ld_cluster_s32(map_to_rank(addr, c)) : 0;
       int total = 0, before = 0;
-#pragma unroll 8
+#pragma unroll
+      for (int c = 0; c < kSortCluster; ++c) {
+        total += n[c];
+        before += c < (int)blockIdx.x ? n[c] : 0;
+      }
+      s_total[x] = total;
+      s_before[x] = before;
+    }
+    __syncwarp();
+    cluster_arrive();                            // waited for at the end: peers may still read this CTA's counts
+  } else if (p.chunk_counts) {
+    const int parts = E < kSortThreads ? kSortThreads / E : 1;
+    const int per = (p.chunks + parts - 1) / parts;
+    for (int i = threadIdx.x; i < parts * E; i += kSortThreads) {
+      const int x = i % E, c0 = i / E * per, c1 = min(c0 + per, p.chunks);
+      int total = 0, before = 0;
+#pragma unroll 16
       for (int c = c0; c < c1; ++c) {
-        const int n = p.chunk_counts[(size_t)c * E + e];
+        const int n = p.chunk_counts[(size_t)c * E + x];
         total += n;
         before += c < (int)blockIdx.x ? n : 0;
       }
-      atomicAdd(s_total + e, total);
-      atomicAdd(s_before + e, before);
+      atomicAdd(s_total + x, total);
+      atomicAdd(s_before + x, before);
     }
+    __syncthreads();
+  } else {
+    for (int x = threadIdx.x; x < E; x += kSortThreads) s_total[x] = s_chunk[x];
   }
-  __syncthreads();
-  int total = 0;
-  if (threadIdx.x < E) {
-    int sum = 0;                                 // counters of a warp become the number of pairs in the warps before it
-    for (int w = 0; w < warps; ++w) {
-      const int n = s_next[w * E + threadIdx.x];
-      s_next[w * E + threadIdx.x] = sum;
-      sum += n;
-    }
-    total = p.chunks > 1 ? s_total[threadIdx.x] : sum;
+  // first rows: a thread has the experts [per x thread, + per); up to kSortThreads experts each has those that it wrote above
+  if (E > kSortThreads) __syncthreads();
+  const int per = (E + kSortThreads - 1) / kSortThreads, x0 = threadIdx.x * per;
+  int padded[kMaxSortExperts / kSortThreads], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kMaxSortExperts / kSortThreads; ++j) {
+    padded[j] = j < per && x0 + j < E ? (s_total[x0 + j] + p.align - 1) / p.align * p.align : 0;
+    sum += padded[j];
   }
-  const int padded = (int)(((long long)total + p.align - 1) / p.align * p.align);
   int used;
-  const int first = block_exclusive_sum(padded, s_warp, &used);
-  if (threadIdx.x < E) {
-    s_total[threadIdx.x] = total;
-    s_first[threadIdx.x] = first;
-    const int base = first + s_before[threadIdx.x];
-    for (int w = 0; w < warps; ++w) s_next[w * E + threadIdx.x] += base;
+  int first = block_exclusive_sum(sum, s_warp, &used);
+#pragma unroll
+  for (int j = 0; j < kMaxSortExperts / kSortThreads; ++j) {
+    if (j >= per || x0 + j >= E) break;
+    s_first[x0 + j] = first;
     if (blockIdx.x == 0) {
-      p.counts[threadIdx.x] = total;
-      p.offsets[threadIdx.x] = first;
+      p.counts[x0 + j] = s_total[x0 + j];
+      p.offsets[x0 + j] = first;
     }
+    first += padded[j];
   }
   if (threadIdx.x == 0) {
     s_first[E] = used;
     if (blockIdx.x == 0) p.offsets[E] = used;
   }
   __syncthreads();
-  if (warp < warps) {
-    int* next = s_next + warp * E;
-    for (long long i0 = begin; i0 < end; i0 += 32) {
-      const long long i = i0 + lane;
-      const int e = i < end ? local_expert(p, i) : -1;
-      const unsigned same = __match_any_sync(0xffffffffu, e);
-      int row = -1;
-      if (e >= 0) row = next[e] + __popc(same & ((1u << lane) - 1u));
-      __syncwarp();
-      if (e >= 0 && lane == 31 - __clz(same)) next[e] = row + 1;
-      __syncwarp();
-      if (i < end) p.pos[i] = row;
-      if (row >= 0) p.pair[row] = (int)i;
-    }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const long long i = first_pair + r * 32;
+    const int row = e[r] >= 0 ? s_first[e[r]] + s_before[e[r]] + mine[e[r]] + rank[r] : -1;
+    if (i < p.pairs) p.pos[i] = row;
+    if (row >= 0) p.pair[row] = (int)i;
   }
   // rows that no pair takes: the padding of every chunks-th expert, and a share of what lies behind the last segment
-  for (int e = (int)blockIdx.x + warp * p.chunks; e < E; e += p.chunks * (blockDim.x >> 5))
-    for (int r = s_first[e] + s_total[e] + lane; r < s_first[e + 1]; r += 32) p.pair[r] = -1;
-  for (long long r = s_first[E] + (long long)blockIdx.x * blockDim.x + threadIdx.x; r < p.rows; r += (long long)p.chunks * blockDim.x)
-    p.pair[r] = -1;
-}
-
-int sort_warps(int e_local) { return e_local <= 256 ? 32 : 16; }
-size_t sort_place_smem(int e_local) { return ((size_t)(sort_warps(e_local) + 3) * e_local + 1 + 32) * 4; }
-
-// One CTA up to kSortOneBlock pairs, else chunks of kSortChunk pairs, larger ones where that makes more CTAs than SMs (every CTA
-// reads the counts of all).
-void sort_chunks(long long pairs, int num_sms, long long* chunk, int* chunks) {
-  if (pairs <= kSortOneBlock) {
-    *chunk = pairs;
-    *chunks = 1;
-    return;
+  if (p.align > 1)
+    for (int x = (int)blockIdx.x + warp * (int)gridDim.x; x < E; x += (int)gridDim.x * kSortWarps)
+      for (int r = s_first[x] + s_total[x] + lane; r < s_first[x + 1]; r += 32) p.pair[r] = -1;
+  long long tail = used;
+  if (p.vec_pair) {                              // (`used` and `rows` are multiples of align, a multiple of four)
+    for (long long r = (long long)used / 4 + (long long)blockIdx.x * kSortThreads + threadIdx.x; r < p.rows / 4; r += (long long)gridDim.x * kSortThreads)
+      reinterpret_cast<int4*>(p.pair)[r] = make_int4(-1, -1, -1, -1);
+    tail = p.rows / 4 * 4;
   }
-  long long c = (pairs + num_sms - 1) / num_sms;
-  c = c < kSortChunk ? kSortChunk : (c + 31) / 32 * 32;
-  *chunk = c;
-  *chunks = (int)((pairs + c - 1) / c);
+  for (long long r = tail + (long long)blockIdx.x * kSortThreads + threadIdx.x; r < p.rows; r += (long long)gridDim.x * kSortThreads)
+    p.pair[r] = -1;
+  __syncwarp();
+  if (cluster) cluster_wait();
 }
-constexpr int kSortMaxChunks = 256;              // more than any sm_100 part has SMs
+
+size_t sort_place_smem(int e_local) { return ((size_t)(kSortWarps + 4) * e_local + 1) * 4; }
+
+// How a number of pairs is sorted: chunks of 512 x `rounds` pairs, in one launch (of one cluster) or in two.
+struct SortPlan {
+  int rounds, chunks;
+  bool one_launch;
+};
+SortPlan sort_plan(long long pairs, long long rows) {
+  constexpr int kSmall = kSortThreads * kSortRounds, kLarge = kSortThreads * kSortManyRounds;
+  SortPlan s;
+  s.one_launch = pairs <= (long long)kSortCluster * kSmall;
+  s.rounds = pairs <= 256ll * kSmall ? kSortRounds : kSortManyRounds;
+  const int chunk = s.rounds == kSortRounds ? kSmall : kLarge;
+  s.chunks = pairs > 0 ? (int)((pairs + chunk - 1) / chunk) : 1;
+  if (s.one_launch) {
+    // clusters of 1, 2, 4, 8; CTAs without pairs where many empty rows are to be marked (16 tokens of 256 experts whose segments
+    // start on multiples of 128: 32640 rows)
+    while (s.chunks < kSortCluster && rows > (long long)s.chunks * 4096) ++s.chunks;
+    while (s.chunks & (s.chunks - 1)) ++s.chunks;
+  }
+  return s;
+}
+
+template <int R>
+cudaError_t launch_sort(const SortParams& p, const SortPlan& plan, cudaStream_t stream) {
+  if (!plan.one_launch) {
+    const cudaError_t e = launch_chained(sort_count_kernel<R>, dim3(plan.chunks), dim3(kSortThreads), (size_t)p.e_local * 4, stream, p);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_chained_cluster(sort_place_kernel<R>, dim3(plan.chunks), dim3(kSortThreads), sort_place_smem(p.e_local), stream,
+                                plan.one_launch ? plan.chunks : 1, p);
+}
 
 // ---- moving rows ----
 
@@ -312,48 +380,67 @@ __device__ __forceinline__ void store_pack(P* p, const P& v) {
 
 constexpr int kSumBatch = 8;                     // rows of a token in flight together
 
-// A warp takes 32 vectors of one token's output row.
-template <typename T, int N>
+// A CTA takes a token's output row, or `segments` CTAs one: the rows' addresses are then known for the whole loop, and eight
+// loads a thread are in flight.  (A warp for each 512 bytes of an output row, which has to fetch the positions first, reached
+// 3.5 TB/s of 14 KB rows.)
+template <typename T, int N, int U>
 __global__ void __launch_bounds__(kMoveThreads)
 unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restrict__ pos, const float* __restrict__ weights,
-                 long long w_stride, T* __restrict__ out, long long out_stride, long long tokens, int top_k, int row_vecs,
-                 int segments) {
+                 long long w_stride, T* __restrict__ out, long long out_stride, int tokens, int top_k, int row_vecs,
+                 int segments, int segment_vecs) {
   using P = Pack<T, N>;
   chain_wait();
   chain_release();
-  const int lane = threadIdx.x & 31;
-  const long long items = tokens * segments, step = (long long)gridDim.x * (kMoveThreads / 32);
-  for (long long w = (long long)blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); w < items; w += step) {
-    const long long t = w / segments;
-    const int v = (int)(w - t * segments) * 32 + lane;
-    const int row_k = lane < top_k ? pos[t * top_k + lane] : -1;
-    const float w_k = weights && lane < top_k ? weights[t * w_stride + lane] : 1.f;
-    float acc[N];
+  const int t = (int)(blockIdx.x / segments), v_begin = (int)(blockIdx.x - (unsigned)t * segments) * segment_vecs;
+  const int v_end = min(v_begin + segment_vecs, row_vecs);
+  const int* at = pos + (size_t)t * top_k;
+  const float* wt = weights ? weights + (size_t)t * w_stride : nullptr;
+  P* dst = reinterpret_cast<P*>(out + (size_t)t * out_stride);
+  const P* src[kSumBatch];
+  float w[kSumBatch];
+  auto rows_from = [&](int k0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = 0.f;
-    for (int k0 = 0; k0 < top_k; k0 += kSumBatch) {
-      P x[kSumBatch];
-#pragma unroll
-      for (int j = 0; j < kSumBatch; ++j) {
-        const int row = __shfl_sync(0xffffffffu, row_k, (k0 + j) & 31);
-        if (k0 + j < top_k && row >= 0 && v < row_vecs)
-          x[j] = load_pack(reinterpret_cast<const P*>(y + (long long)row * y_stride) + v);
-      }
-#pragma unroll
-      for (int j = 0; j < kSumBatch; ++j) {
-        const int row = __shfl_sync(0xffffffffu, row_k, (k0 + j) & 31);
-        const float wt = __shfl_sync(0xffffffffu, w_k, (k0 + j) & 31);
-        if (k0 + j < top_k && row >= 0) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) acc[i] = fmaf(wt, to_float(x[j].v[i]), acc[i]);
-        }
-      }
+    for (int j = 0; j < kSumBatch; ++j) {
+      const int row = k0 + j < top_k ? __ldg(at + k0 + j) : -1;
+      src[j] = row >= 0 ? reinterpret_cast<const P*>(y + row * y_stride) : nullptr;
+      w[j] = wt && k0 + j < top_k ? __ldg(wt + k0 + j) : 1.f;
     }
-    if (v < row_vecs) {
+  };
+  rows_from(0);
+  for (int v = v_begin + threadIdx.x; v < v_end; v += U * kMoveThreads) {
+    float acc[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
+    for (int k0 = 0;;) {
+      P x[kSumBatch][U];
+#pragma unroll
+      for (int j = 0; j < kSumBatch; ++j)
+        if (src[j]) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (U == 1 || v + u * kMoveThreads < v_end) x[j][u] = load_pack(src[j] + v + u * kMoveThreads);
+        }
+#pragma unroll
+      for (int j = 0; j < kSumBatch; ++j)
+        if (src[j]) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[u][i] = fmaf(w[j], to_float(x[j][u].v[i]), acc[u][i]);
+        }
+      if (top_k <= kSumBatch) break;
+      k0 = k0 + kSumBatch < top_k ? k0 + kSumBatch : 0;   // (more choices: the next eight, and the first again for the next v)
+      rows_from(k0);
+      if (k0 == 0) break;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       P r;
 #pragma unroll
-      for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(acc[i]);
-      store_pack(reinterpret_cast<P*>(out + t * out_stride) + v, r);
+      for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(acc[u][i]);
+      if (U == 1 || v + u * kMoveThreads < v_end) store_pack(dst + v + u * kMoveThreads, r);
     }
   }
 }
@@ -379,7 +466,7 @@ struct UnpermuteGrad {
 // One CTA per token: its row of dout is read once (top_k <= 8), each sorted row of y read and of dy written once; the dots are
 // summed by shuffles and over the four warps in a fixed order.
 template <typename T, int N>
-__global__ void __launch_bounds__(kMoveThreads)
+__global__ void __launch_bounds__(kMoveThreads, 5)
 unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long items) {
   using P = Pack<T, N>;
   constexpr int kWarps = kMoveThreads / 32;
@@ -446,18 +533,13 @@ unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long item
   }
 }
 
-bool aligned16(const void* p, long long stride_bytes) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride_bytes % 16 == 0;
-}
-
 unsigned grid_for(long long items, long long most) { return (unsigned)(items < most ? items : most); }
 
 template <typename V, int U>
-cudaError_t launch_permute_rows(const RowMove& p, bool zero, int num_sms, cudaStream_t stream) {
+cudaError_t launch_permute_rows(const RowMove& p, int num_sms, cudaStream_t stream) {
   const int segments = (p.row_vecs + U * 32 - 1) / (U * 32);
   const long long move_items = p.tokens * segments;
-  const long long items = move_items + (zero ? (p.rows + kZeroRows - 1) / kZeroRows : 0);
-  if (items == 0) return cudaSuccess;
+  const long long items = move_items + (p.rows + kZeroRows - 1) / kZeroRows;
   constexpr int kWarps = kMoveThreads / 32;
   return launch_chained(permute_kernel<V, U>, dim3(grid_for((items + kWarps - 1) / kWarps, 64ll * num_sms)), dim3(kMoveThreads), 0,
                         stream, p, segments, move_items, items);
@@ -465,22 +547,36 @@ cudaError_t launch_permute_rows(const RowMove& p, bool zero, int num_sms, cudaSt
 
 template <typename T, int N>
 cudaError_t launch_unpermute(const void* y, long long y_stride, const int* pos, const float* weights, long long w_stride, void* out,
-                             long long out_stride, long long tokens, int top_k, int hidden, int num_sms, cudaStream_t stream) {
-  const int row_vecs = hidden / N, segments = (row_vecs + 31) / 32;
-  constexpr int kWarps = kMoveThreads / 32;
-  const long long blocks = (tokens * segments + kWarps - 1) / kWarps;
-  return launch_chained(unpermute_kernel<T, N>, dim3(grid_for(blocks, 64ll * num_sms)), dim3(kMoveThreads), 0, stream,
+                             long long out_stride, int tokens, int top_k, int hidden, int num_sms, cudaStream_t stream) {
+  constexpr int U = sizeof(T) * N == 16 ? 1 : sizeof(T) * N == 4 ? 2 : 4;   // loads of fewer bytes: more of them in flight
+  const int row_vecs = hidden / N;
+  // one CTA a token, more where that leaves SMs without one
+  const int pieces = (row_vecs + kMoveThreads - 1) / kMoveThreads;
+  int segments = (int)((8ll * num_sms + tokens - 1) / tokens);
+  if (segments > pieces) segments = pieces;
+  const int segment_vecs = (pieces + segments - 1) / segments * kMoveThreads;
+  segments = (row_vecs + segment_vecs - 1) / segment_vecs;
+  if ((long long)tokens * segments > 0x7fffffffll) return cudaErrorInvalidValue;
+  return launch_chained(unpermute_kernel<T, N, U>, dim3((unsigned)tokens * segments), dim3(kMoveThreads), 0, stream,
                         reinterpret_cast<const T*>(y), y_stride, pos, weights, w_stride, reinterpret_cast<T*>(out), out_stride,
-                        tokens, top_k, row_vecs, segments);
+                        tokens, top_k, row_vecs, segments, segment_vecs);
+}
+
+// elements of a vector: 16 bytes, 4 bytes or one element, as far as all rows start on such a boundary (`bits`: addresses
+// and pitches in bytes, or'ed)
+template <typename T> int vector_elems(int hidden, uintptr_t bits) {
+  const uintptr_t row = (uintptr_t)hidden * sizeof(T) | bits;
+  return row % 16 == 0 ? 16 / (int)sizeof(T) : row % 4 == 0 ? 4 / (int)sizeof(T) : 1;
 }
 
 template <typename T>
 cudaError_t unpermute_type(const void* y, long long y_stride, const int* pos, const float* weights, long long w_stride, void* out,
-                           long long out_stride, long long tokens, int top_k, int hidden, int num_sms, cudaStream_t stream) {
-  constexpr int N = 16 / sizeof(T);
-  const bool vec = hidden % N == 0 && aligned16(y, y_stride * (long long)sizeof(T)) && aligned16(out, out_stride * (long long)sizeof(T));
-  return vec ? launch_unpermute<T, N>(y, y_stride, pos, weights, w_stride, out, out_stride, tokens, top_k, hidden, num_sms, stream)
-             : launch_unpermute<T, 1>(y, y_stride, pos, weights, w_stride, out, out_stride, tokens, top_k, hidden, num_sms, stream);
+                           long long out_stride, int tokens, int top_k, int hidden, int num_sms, cudaStream_t stream) {
+  constexpr int N16 = 16 / sizeof(T), N4 = 4 / sizeof(T);
+  const int n = vector_elems<T>(hidden, reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out) |
+                                            (uintptr_t)(y_stride * sizeof(T)) | (uintptr_t)(out_stride * sizeof(T)));
+  auto go = n == N16 ? launch_unpermute<T, N16> : n == N4 ? launch_unpermute<T, N4> : launch_unpermute<T, 1>;
+  return go(y, y_stride, pos, weights, w_stride, out, out_stride, tokens, top_k, hidden, num_sms, stream);
 }
 
 template <typename T, int N>
@@ -514,11 +610,13 @@ cudaError_t unpermute_grad_type(const void* dout, long long dout_stride, const v
   p.rows = rows;
   p.top_k = top_k;
   p.row_vecs = 0;
-  constexpr int N = 16 / sizeof(T);
-  const long long b = sizeof(T);
-  const bool vec = hidden % N == 0 && aligned16(dout, dout_stride * b) && (!dw || aligned16(y, y_stride * b)) &&
-                   (!dy || aligned16(dy, dy_stride * b));
-  return vec ? launch_unpermute_grad<T, N>(p, hidden, num_sms, stream) : launch_unpermute_grad<T, 1>(p, hidden, num_sms, stream);
+  constexpr int N16 = 16 / sizeof(T), N4 = 4 / sizeof(T);
+  uintptr_t bits = reinterpret_cast<uintptr_t>(dout) | (uintptr_t)(dout_stride * sizeof(T));
+  if (dw) bits |= reinterpret_cast<uintptr_t>(y) | (uintptr_t)(y_stride * sizeof(T));
+  if (dy) bits |= reinterpret_cast<uintptr_t>(dy) | (uintptr_t)(dy_stride * sizeof(T));
+  const int n = vector_elems<T>(hidden, bits);
+  auto go = n == N16 ? launch_unpermute_grad<T, N16> : n == N4 ? launch_unpermute_grad<T, N4> : launch_unpermute_grad<T, 1>;
+  return go(p, hidden, num_sms, stream);
 }
 
 // tokens x top_k pairs and `rows` sorted rows that int32 tables can name
@@ -531,7 +629,10 @@ int order_ok(int64_t tokens, int top_k, int64_t rows) {
 }  // namespace
 
 cudaError_t configure_sort_rows() {
-  return cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sort_place_smem(kMaxSortExperts));
+  const int bytes = (int)sort_place_smem(kMaxSortExperts);
+  const cudaError_t e = cudaFuncSetAttribute(sort_place_kernel<kSortRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(sort_place_kernel<kSortManyRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 }  // namespace b200moe
@@ -548,9 +649,10 @@ int64_t b200moe_sort_rows(int64_t tokens, int top_k, int e_local, int align) {
   return (rows + align - 1) / align * align;
 }
 
-int64_t b200moe_sort_workspace_bytes(int e_local) {
-  if (e_local < 1 || e_local > kMaxSortExperts) return B200MOE_ERR_INVALID_ARGUMENT;
-  return (int64_t)kSortMaxChunks * e_local * 4;
+int64_t b200moe_sort_workspace_bytes(int64_t tokens, int top_k, int e_local) {
+  if (order_ok(tokens, top_k, 0) != B200MOE_OK || e_local < 1 || e_local > kMaxSortExperts) return B200MOE_ERR_INVALID_ARGUMENT;
+  const SortPlan plan = sort_plan(tokens * top_k, 0);
+  return plan.one_launch ? 0 : (int64_t)plan.chunks * e_local * 4;
 }
 
 int b200moe_sort_tokens(const void* topk_ids, int ids_bits, int64_t ids_row_stride, int64_t tokens, int top_k, int e_local,
@@ -567,32 +669,33 @@ int b200moe_sort_tokens(const void* topk_ids, int ids_bits, int64_t ids_row_stri
   if (rows > 0 && !pair) return B200MOE_ERR_INVALID_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(topk_ids) % (ids_bits / 8) != 0 || reinterpret_cast<uintptr_t>(workspace) % 4 != 0)
     return B200MOE_ERR_MISALIGNED;
+  const SortPlan plan = sort_plan(tokens * top_k, rows);
+  if (!plan.one_launch) {
+    if (!workspace) return B200MOE_ERR_INVALID_ARGUMENT;
+    if (workspace_bytes < (size_t)plan.chunks * e_local * 4) return B200MOE_ERR_WORKSPACE_TOO_SMALL;
+  }
   int num_sms = 0;
   if ((rc = ensure_device(&num_sms)) != B200MOE_OK) return rc;
   SortParams p;
   p.ids = topk_ids;
   p.ids_stride = ids_row_stride;
-  p.pairs = tokens * top_k;
+  p.pairs = (int)(tokens * top_k);
   p.top_k = top_k;
+  p.contiguous = ids_row_stride == top_k || tokens <= 1;
   p.wide = ids_bits == 64;
+  p.vec_pair = align % 4 == 0 && reinterpret_cast<uintptr_t>(pair) % 16 == 0;
   p.local_off = local_expert_offset;
   p.e_local = e_local;
   p.align = align;
-  p.rows = rows;
+  p.rows = (int)rows;
   p.counts = counts;
   p.offsets = offsets;
   p.pos = pos;
   p.pair = pair;
-  p.chunk_counts = reinterpret_cast<int*>(workspace);
-  sort_chunks(p.pairs, num_sms < kSortMaxChunks ? num_sms : kSortMaxChunks, &p.chunk, &p.chunks);
+  p.chunks = plan.chunks;
+  p.chunk_counts = plan.one_launch ? nullptr : reinterpret_cast<int*>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (p.chunks > 1) {
-    if (!workspace) return B200MOE_ERR_INVALID_ARGUMENT;
-    if (workspace_bytes < (size_t)p.chunks * e_local * 4) return B200MOE_ERR_WORKSPACE_TOO_SMALL;
-    CUDA_TRY(launch_chained(sort_count_kernel, dim3(p.chunks), dim3(kSortThreads), (size_t)e_local * 4, st, p));
-  }
-  CUDA_TRY(launch_chained(sort_place_kernel, dim3(p.chunks), dim3(kSortThreads), sort_place_smem(e_local), st, p,
-                          sort_warps(e_local)));
+  CUDA_TRY(plan.rounds == kSortRounds ? launch_sort<kSortRounds>(p, plan, st) : launch_sort<kSortManyRounds>(p, plan, st));
   return B200MOE_OK;
 }
 
@@ -624,16 +727,19 @@ int b200moe_permute_rows(const void* x, int64_t x_row_bytes, int64_t row_bytes, 
   p.rows = rows;
   p.top_k = top_k;
   p.zero_tail = zero_tail != 0;
-  const bool vec = row_bytes % 16 == 0 && aligned16(x, x_row_bytes) && aligned16(y, y_row_bytes);
-  p.row_vecs = (int)(row_bytes / (vec ? 16 : elem_bytes));
-  if (vec)
-    CUDA_TRY((launch_permute_rows<uint4, 1>(p, true, num_sms, st)));
-  else if (elem_bytes == 4)
-    CUDA_TRY((launch_permute_rows<uint32_t, 4>(p, true, num_sms, st)));
-  else if (elem_bytes == 2)
-    CUDA_TRY((launch_permute_rows<uint16_t, 4>(p, true, num_sms, st)));
+  // what a lane moves at once: 16 bytes, or the largest smaller part on whose boundaries all rows start
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | (uintptr_t)x_row_bytes | reinterpret_cast<uintptr_t>(y) |
+                         (uintptr_t)y_row_bytes | (uintptr_t)row_bytes;
+  const int vec = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+  p.row_vecs = (int)(row_bytes / vec);
+  if (vec == 16)
+    CUDA_TRY((launch_permute_rows<uint4, 1>(p, num_sms, st)));
+  else if (vec == 4)
+    CUDA_TRY((launch_permute_rows<uint32_t, 4>(p, num_sms, st)));
+  else if (vec == 2)
+    CUDA_TRY((launch_permute_rows<uint16_t, 8>(p, num_sms, st)));
   else
-    CUDA_TRY((launch_permute_rows<uint8_t, 4>(p, true, num_sms, st)));
+    CUDA_TRY((launch_permute_rows<uint8_t, 8>(p, num_sms, st)));
   return B200MOE_OK;
 }
 
@@ -652,7 +758,7 @@ int b200moe_unpermute_rows(const void* y, int dtype, int64_t y_row_stride, const
   if ((rc = ensure_device(&num_sms)) != B200MOE_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto go = dtype == B200MOE_F32 ? unpermute_type<float> : dtype == B200MOE_BF16 ? unpermute_type<__nv_bfloat16> : unpermute_type<__half>;
-  CUDA_TRY(go(y, y_row_stride, pos, weights, w_row_stride, out, out_row_stride, tokens, top_k, hidden, num_sms, st));
+  CUDA_TRY(go(y, y_row_stride, pos, weights, w_row_stride, out, out_row_stride, (int)tokens, top_k, hidden, num_sms, st));
   return B200MOE_OK;
 }
 

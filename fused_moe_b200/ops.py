@@ -13,7 +13,7 @@ weight format, and tokens sorted by expert and back.
 The layer from parts is the sequence route, sort_tokens, permute, quantize, block_matmul per expert, quantize with SwiGLU,
 block_matmul, unpermute.  All results repeat bit for bit (there are no atomics on values), every call is asynchronous on the
 current stream of its tensors' device, can be captured into a CUDA graph and allocates only its results (and the sort, above
-8192 pairs, a scratch tensor) from torch's allocator.  Errors: ``TypeError`` / ``ValueError`` for arguments, ``RuntimeError``
+16384 pairs, a scratch tensor) from torch's allocator.  Errors: ``TypeError`` / ``ValueError`` for arguments, ``RuntimeError``
 for tensors that are not on one CUDA device, ``MoEError`` for what the library refuses.
 
 The reference has no counterparts: its only public function is the fused layer (solution/python/kernel.py:642-648).
@@ -29,6 +29,7 @@ from . import _capi
 from ._capi import MoEError
 from .kernel import BLOCK, E_GLOBAL, _as_bytes
 
+_SORT_ONE_LAUNCH = 16384      # pairs that the sort handles without a scratch tensor
 _DTYPE = {torch.float32: _capi.F32, torch.bfloat16: _capi.BF16, torch.float16: _capi.F16}
 
 
@@ -270,8 +271,8 @@ def sort_tokens(topk_ids: torch.Tensor, e_local: int = E_GLOBAL, local_expert_of
     with _on(dev) as stream:
         lib = _capi.lib()
         ws, ws_bytes, ws_ptr = None, 0, None
-        if pairs > 8192:
-            ws_bytes = lib.b200moe_sort_workspace_bytes(e_local)
+        if pairs > _SORT_ONE_LAUNCH:
+            ws_bytes = lib.b200moe_sort_workspace_bytes(tokens, top_k, e_local)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
             ws_ptr = ws.data_ptr()
         rc = lib.b200moe_sort_tokens(ids.data_ptr(), ids.element_size() * 8, _pitch(ids), tokens, top_k, e_local, off, align,

@@ -303,8 +303,8 @@ B200MOE_API int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride,
  * Negative: a status (bad argument). */
 B200MOE_API int64_t b200moe_sort_rows(int64_t tokens, int top_k, int e_local, int align);
 
-/* Bytes of workspace that b200moe_sort_tokens needs for any number of tokens.  Negative: a status. */
-B200MOE_API int64_t b200moe_sort_workspace_bytes(int e_local);
+/* Bytes of workspace that b200moe_sort_tokens needs (0 up to 16384 pairs).  Negative: a status. */
+B200MOE_API int64_t b200moe_sort_workspace_bytes(int64_t tokens, int top_k, int e_local);
 
 /* Stable sort of the pairs (t, k) by expert.  ids of `ids_bits` 32 or 64, `ids_row_stride` elements; an id outside
  * [local_expert_offset, local_expert_offset + e_local) is not local and gets no row; an expert that a token names twice gets
@@ -314,7 +314,7 @@ B200MOE_API int64_t b200moe_sort_workspace_bytes(int e_local);
  *  pos      int32[tokens][top_k] row of each pair, -1: not local
  *  pair     int32[rows]         t*top_k + k of each row, -1: padding, or behind the last segment
  *  rows     length of `pair`, at least b200moe_sort_rows(...)
- *  workspace may be NULL up to 8192 pairs. */
+ *  workspace may be NULL where b200moe_sort_workspace_bytes is 0. */
 B200MOE_API int b200moe_sort_tokens(const void* topk_ids, int ids_bits, int64_t ids_row_stride, int64_t tokens, int top_k,
                         int e_local, int local_expert_offset, int align,
                         int32_t* counts, int32_t* offsets, int32_t* pos, int32_t* pair, int64_t rows,

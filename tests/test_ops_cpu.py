@@ -81,7 +81,12 @@ def test_sort_refusals(mem):
     assert lib.b200moe_sort_rows(1, 2, 16, 128) == 256                  # two pairs: two segments at most
     assert lib.b200moe_sort_rows(0, 2, 16, 128) == 0
     assert lib.b200moe_sort_rows(4, 33, 16, 1) == INVALID and lib.b200moe_sort_rows(4, 8, 0, 1) == INVALID
-    assert lib.b200moe_sort_workspace_bytes(0) == INVALID and lib.b200moe_sort_workspace_bytes(256) == 256 * 256 * 4
+    assert lib.b200moe_sort_workspace_bytes(4, 8, 0) == INVALID and lib.b200moe_sort_workspace_bytes(4, 33, 8) == INVALID
+    # none up to the pairs that one launch sorts (the host allocates none either), then a histogram for each chunk
+    assert lib.b200moe_sort_workspace_bytes(2048, 8, 256) == 0 and F.ops._SORT_ONE_LAUNCH == 2048 * 8
+    assert lib.b200moe_sort_workspace_bytes(2049, 8, 256) == 9 * 256 * 4
+    assert lib.b200moe_sort_workspace_bytes(65537, 8, 10) == -(-65537 * 8 // 8192) * 10 * 4
+    assert call(_3=3000, _12=24000) == INVALID and call(_3=3000, _12=24000, _13=p, _14=12 * 16 * 4 - 1) == SPACE
 
 
 def test_row_moves_refusals(mem):
