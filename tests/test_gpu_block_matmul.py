@@ -12,7 +12,8 @@ HALF_ULP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32:
 
 SHAPES = [(1, 1, 16), (1, 128, 128), (2, 130, 144), (7, 64, 272), (8, 4096, 7168), (9, 1000, 1024), (16, 512, 2048), (17, 129, 400),
           (33, 257, 1168), (64, 7168, 2048), (65, 300, 640), (127, 384, 4096), (128, 128, 128), (129, 513, 256), (200, 1001, 7168),
-          (256, 576, 1536), (300, 2048, 512), (511, 255, 2064), (1025, 1152, 896), (2048, 2304, 1024), (4100, 520, 384)]
+          (256, 576, 1536), (300, 2048, 512), (511, 255, 2064), (1025, 1152, 896), (2048, 2304, 1024), (4100, 520, 384),
+          (129, 7168, 16384), (4200, 4224, 400), (2500, 5000, 1936)]
 
 
 def expand(sa, sb, N, K):
