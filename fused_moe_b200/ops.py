@@ -27,32 +27,28 @@ import torch
 
 from . import _capi
 from ._capi import MoEError
-from .kernel import BLOCK, E_GLOBAL, _as_bytes
+from .kernel import BLOCK, E_GLOBAL
 
 _SORT_ONE_LAUNCH = 16384      # pairs that the sort handles without a scratch tensor
+_CODES = (torch.float8_e4m3fn, torch.uint8)
 _DTYPE = {torch.float32: _capi.F32, torch.bfloat16: _capi.BF16, torch.float16: _capi.F16}
 
 
-class _on:
-    """The device of a call's tensors, current while the call is made, and its current stream."""
+# what a call asks of torch besides its tensors, without the Python layers above: half a microsecond instead of four
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-    __slots__ = ("device", "before", "stream")
 
-    def __init__(self, device: torch.device):
-        self.device = device
-
-    def __enter__(self):
-        index = self.device.index
-        self.before = torch.cuda.current_device()
-        if self.before != index:
-            torch.cuda.set_device(index)
-        self.stream = torch.cuda.current_stream(index).cuda_stream
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.before)
-        return False
+def _call(name: str, index: int, *args) -> None:
+    """Library call with its device current, on that device's current stream (the last argument)."""
+    fn = getattr(_capi.lib(), name)
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _capi.check(rc, name)
 
 
 def _cuda(t: torch.Tensor, what: str) -> torch.device:
@@ -61,10 +57,10 @@ def _cuda(t: torch.Tensor, what: str) -> torch.device:
     return t.device
 
 
-def _same_device(dev: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{name} is on {t.device}, the other arguments on {dev}")
+def _other_device(dev: torch.device, **tensors) -> RuntimeError:
+    """The error for arguments of which one is not on ``dev``."""
+    name, t = next((n, t) for n, t in tensors.items() if t is not None and t.device != dev)
+    return RuntimeError(f"{name} is on {t.device}, the other arguments on {dev}")
 
 
 def _no_grad(what: str, *tensors) -> None:
@@ -78,6 +74,8 @@ def _rows2d(t: torch.Tensor, what: str) -> torch.Tensor:
     """``t`` with unit inner stride and rows that do not overlap (a copy where it has not)."""
     if t.dim() != 2:
         raise ValueError(f"{what} must be 2-D, got shape {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t
     if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
@@ -121,15 +119,14 @@ def quantize(x: torch.Tensor, *, swiglu: bool = False, scale_layout: str = "kt")
             raise ValueError(f"swiglu needs an even number of columns (gate half, up half), got {cols}")
         cols //= 2
     blocks = -(-cols // BLOCK)
-    codes = torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=dev)
-    kt = scale_layout == "kt"
-    scale = torch.empty((blocks, rows) if kt else (rows, blocks), dtype=torch.float32, device=dev)
-    if rows == 0 or cols == 0:
-        return codes, scale
-    with _on(dev) as stream:
-        rc = _capi.lib().b200moe_quantize(x.data_ptr(), dt, _pitch(x), rows, cols, int(swiglu), codes.data_ptr(), cols,
-                                          scale.data_ptr(), 1 if kt else blocks, rows if kt else 1, stream)
-    _capi.check(rc, "b200moe_quantize")
+    codes = torch.empty(rows, cols, dtype=torch.float8_e4m3fn, device=dev)
+    if scale_layout == "kt":
+        scale, stride_t, stride_kb = torch.empty(blocks, rows, dtype=torch.float32, device=dev), 1, rows
+    else:
+        scale, stride_t, stride_kb = torch.empty(rows, blocks, dtype=torch.float32, device=dev), blocks, 1
+    if rows and cols:
+        _call("b200moe_quantize", dev.index, x.data_ptr(), dt, _pitch(x), rows, cols, int(swiglu), codes.data_ptr(), cols,
+              scale.data_ptr(), stride_t, stride_kb)
     return codes, scale
 
 
@@ -155,13 +152,15 @@ _status: Dict[int, _Status] = {}
 
 def _block_scale_strides(scale: torch.Tensor, rows: int, blocks: int, layout: str, what: str) -> Tuple[int, int]:
     """(stride over rows, stride over K blocks) of a scale tensor, in elements."""
-    want = (blocks, rows) if layout == "kt" else (rows, blocks)
     if scale.dtype != torch.float32:
         raise TypeError(f"{what} must be float32, got {scale.dtype}")
-    if tuple(scale.shape) != want:
-        raise ValueError(f"{what} has shape {tuple(scale.shape)}, expected {want} for scale_layout {layout!r}")
-    s0, s1 = scale.stride()
-    return (s1, s0) if layout == "kt" else (s0, s1)
+    if layout == "kt":
+        if scale.shape == (blocks, rows):
+            return scale.stride()[::-1]
+    elif scale.shape == (rows, blocks):
+        return scale.stride()
+    want = (blocks, rows) if layout == "kt" else (rows, blocks)
+    raise ValueError(f"{what} has shape {tuple(scale.shape)}, expected {want} for scale_layout {layout!r}")
 
 
 def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, *, scale_layout: str = "kt",
@@ -175,12 +174,17 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     (which must not overlap the inputs).  Not differentiable: the operands are codes.
     """
     dev = _cuda(a, "a")
-    _same_device(dev, a_scale=a_scale, b=b, b_scale=b_scale)
+    if a_scale.device != dev or b.device != dev or b_scale.device != dev:
+        raise _other_device(dev, a_scale=a_scale, b=b, b_scale=b_scale)
     _no_grad("block_matmul", a_scale, b_scale)
-    a, b = _rows2d(_as_bytes(a, "a"), "a"), _as_bytes(b, "b")
-    if b.dim() != 2 or b.shape[1] != a.shape[1]:
-        raise ValueError(f"b must be [N, {a.shape[1]}], got {tuple(b.shape)}")
-    (M, K), N = a.shape, b.shape[0]
+    for name, t in (("a", a), ("b", b)):
+        if t.dtype not in _CODES:
+            raise TypeError(f"{name} must be float8_e4m3fn (or its uint8 bit pattern), got {t.dtype}")
+    a = _rows2d(a, "a")
+    M, K = a.shape
+    if b.dim() != 2 or b.shape[1] != K:
+        raise ValueError(f"b must be [N, {K}], got {tuple(b.shape)}")
+    N = b.shape[0]
     if K == 0 or K % 16:
         raise ValueError(f"K must be a positive multiple of 16, got {K}")
     if scale_layout not in ("kt", "tk"):
@@ -188,15 +192,17 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     blocks = -(-K // BLOCK)
     as_m, as_kb = _block_scale_strides(a_scale, M, blocks, scale_layout, "a_scale")
     bs_n, bs_kb = _block_scale_strides(b_scale, -(-N // BLOCK), blocks, "tk", "b_scale")
-    if b.stride(1) != 1 or (N > 1 and (b.stride(0) < K or b.stride(0) % 16)) or b.data_ptr() % 16:
+    a_ptr, a_pitch, b_ptr, b_pitch = a.data_ptr(), _pitch(a), b.data_ptr(), _pitch(b)
+    if (b_ptr | b_pitch) % 16 or b_pitch < K or b.stride(1) != 1:
         raise ValueError("b must have unit inner stride and rows on 16-byte boundaries")
-    if _pitch(a) % 16 or a.data_ptr() % 16:
-        a = a.contiguous() if a.data_ptr() % 16 == 0 and not a.is_contiguous() else a.clone(memory_format=torch.contiguous_format)
+    if (a_ptr | a_pitch) % 16:
+        a = a.clone(memory_format=torch.contiguous_format)
+        a_ptr, a_pitch = a.data_ptr(), K
     if out is None:
         dt = _DTYPE.get(out_dtype)
         if dt is None:
             raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
-        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+        out = torch.empty(M, N, dtype=out_dtype, device=dev)
     else:
         dt = _DTYPE.get(out.dtype)
         if dt is None:
@@ -209,18 +215,15 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
         st = _status[dev.index] = _Status()
     if st is not None:
         st.raise_if_failed()
-    with _on(dev) as stream:
-        rc = _capi.lib().b200moe_block_matmul(a.data_ptr(), _pitch(a), a_scale.data_ptr(), as_m, as_kb, b.data_ptr(), _pitch(b),
-                                              b_scale.data_ptr(), bs_n, bs_kb, M, N, K, out.data_ptr(), dt, _pitch(out),
-                                              None if st is None else st.ptr, stream)
-    _capi.check(rc, "b200moe_block_matmul")
+    _call("b200moe_block_matmul", dev.index, a_ptr, a_pitch, a_scale.data_ptr(), as_m, as_kb, b_ptr, b_pitch, b_scale.data_ptr(),
+          bs_n, bs_kb, M, N, K, out.data_ptr(), dt, _pitch(out), None if st is None else st.ptr)
     return out
 
 
 # ---- tokens sorted by expert and back ----
 
 class TokenOrder:
-    """What ``sort_tokens`` found; int32 tensors on the ids' device.
+    """What ``sort_tokens`` found; int32 tensors on the ids' device (views of one, made when they are asked for).
 
     offsets [e_local + 1]  first row of each local expert, the last: rows in use
     counts  [e_local]      pairs of each local expert
@@ -228,13 +231,37 @@ class TokenOrder:
     pair    [rows]         token * top_k + k of each row, -1 in padding and behind the last expert
     """
 
-    __slots__ = ("offsets", "counts", "pos", "pair", "tokens", "top_k", "rows", "e_local", "local_expert_offset", "align")
+    __slots__ = ("tokens", "top_k", "rows", "e_local", "local_expert_offset", "align", "device", "_table", "_pos_at", "_pair_at", "_ptr")
 
-    def __init__(self, offsets, counts, pos, pair, e_local, local_expert_offset, align):
-        self.offsets, self.counts, self.pos, self.pair = offsets, counts, pos, pair
-        self.tokens, self.top_k = pos.shape
-        self.rows = pair.shape[0]
+    def __init__(self, device, tokens, top_k, rows, e_local, local_expert_offset, align):
+        self.device, self.tokens, self.top_k, self.rows = device, tokens, top_k, rows
         self.e_local, self.local_expert_offset, self.align = e_local, local_expert_offset, align
+        # offsets, counts, pos, pair: the latter two at multiples of 16 bytes
+        self._pos_at = (2 * e_local + 4) // 4 * 4
+        self._pair_at = self._pos_at + (tokens * top_k + 3) // 4 * 4
+        self._table = torch.empty(self._pair_at + rows, dtype=torch.int32, device=device)
+        self._ptr = self._table.data_ptr()
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        return self._table[:self.e_local + 1]
+
+    @property
+    def counts(self) -> torch.Tensor:
+        return self._table[self.e_local + 1:2 * self.e_local + 1]
+
+    @property
+    def pos(self) -> torch.Tensor:
+        return self._table.as_strided((self.tokens, self.top_k), (self.top_k, 1), self._pos_at)
+
+    @property
+    def pair(self) -> torch.Tensor:
+        return self._table[self._pair_at:]
+
+    @property
+    def _pointers(self) -> Tuple[int, int, int]:
+        """Addresses of pos, pair and offsets."""
+        return self._ptr + 4 * self._pos_at, self._ptr + 4 * self._pair_at, self._ptr
 
 
 def sort_tokens(topk_ids: torch.Tensor, e_local: int = E_GLOBAL, local_expert_offset: int = 0, *, align: int = 1) -> TokenOrder:
@@ -262,48 +289,36 @@ def sort_tokens(topk_ids: torch.Tensor, e_local: int = E_GLOBAL, local_expert_of
     rows = -(-(pairs + (align - 1) * min(pairs, e_local)) // align) * align
     if rows >= 2 ** 31:
         raise ValueError(f"{rows} sorted rows: int32 tables name at most {2 ** 31 - 1}")
-    # one allocation, the four tables each at a multiple of 16 bytes
-    pos_at = (2 * e_local + 1 + 3) // 4 * 4
-    pair_at = pos_at + (pairs + 3) // 4 * 4
-    table = torch.empty(pair_at + rows, dtype=torch.int32, device=dev)
-    offsets, counts = table[:e_local + 1], table[e_local + 1:2 * e_local + 1]
-    pos, pair = table[pos_at:pos_at + pairs].view(tokens, top_k), table[pair_at:]
-    with _on(dev) as stream:
-        lib = _capi.lib()
-        ws, ws_bytes, ws_ptr = None, 0, None
-        if pairs > _SORT_ONE_LAUNCH:
-            ws_bytes = lib.b200moe_sort_workspace_bytes(tokens, top_k, e_local)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            ws_ptr = ws.data_ptr()
-        rc = lib.b200moe_sort_tokens(ids.data_ptr(), ids.element_size() * 8, _pitch(ids), tokens, top_k, e_local, off, align,
-                                     counts.data_ptr(), offsets.data_ptr(), pos.data_ptr(), pair.data_ptr(), rows,
-                                     ws_ptr, ws_bytes, stream)
-    _capi.check(rc, "b200moe_sort_tokens")
-    return TokenOrder(offsets, counts, pos, pair, e_local, off, align)
+    order = TokenOrder(dev, tokens, top_k, rows, e_local, off, align)
+    ws, ws_bytes = None, 0
+    if pairs > _SORT_ONE_LAUNCH:
+        ws_bytes = _capi.lib().b200moe_sort_workspace_bytes(tokens, top_k, e_local)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    pos, pair, offsets = order._pointers
+    _call("b200moe_sort_tokens", dev.index, ids.data_ptr(), ids.element_size() * 8, _pitch(ids), tokens, top_k, e_local, off, align,
+          offsets + 4 * (e_local + 1), offsets, pos, pair, rows, None if ws is None else ws.data_ptr(), ws_bytes)
+    return order
 
 
 def _permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor]) -> torch.Tensor:
-    dev, size, H = x.device, x.element_size(), x.shape[1]
     x = _rows2d(x, "x")
-    y = torch.empty((order.rows, H), dtype=x.dtype, device=dev) if out is None else out
-    with _on(dev) as stream:
-        rc = _capi.lib().b200moe_permute_rows(x.data_ptr(), _pitch(x) * size, H * size, size, order.tokens, order.top_k,
-                                              order.pos.data_ptr(), order.pair.data_ptr(), order.offsets.data_ptr(),
-                                              order.e_local, order.rows, y.data_ptr(), _pitch(y) * size, int(out is None), stream)
-    _capi.check(rc, "b200moe_permute_rows")
+    dev, size, H = x.device, x.element_size(), x.shape[1]
+    y = torch.empty(order.rows, H, dtype=x.dtype, device=dev) if out is None else out
+    _call("b200moe_permute_rows", dev.index, x.data_ptr(), _pitch(x) * size, H * size, size, order.tokens, order.top_k,
+          *order._pointers, order.e_local, order.rows, y.data_ptr(), _pitch(y) * size, int(out is None))
     return y
 
 
 def _unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tensor], out: Optional[torch.Tensor]) -> torch.Tensor:
-    dev, H = y.device, y.shape[1]
     y = _rows2d(y, "y")
-    w = None if weights is None else _rows2d(weights, "weights")
-    res = torch.empty((order.tokens, H), dtype=y.dtype, device=dev) if out is None else out
-    with _on(dev) as stream:
-        rc = _capi.lib().b200moe_unpermute_rows(y.data_ptr(), _DTYPE[y.dtype], _pitch(y), order.pos.data_ptr(),
-                                                None if w is None else w.data_ptr(), 0 if w is None else _pitch(w),
-                                                order.tokens, order.top_k, H, res.data_ptr(), _pitch(res), stream)
-    _capi.check(rc, "b200moe_unpermute_rows")
+    dev, H = y.device, y.shape[1]
+    w_ptr, w_pitch = None, 0
+    if weights is not None:
+        weights = _rows2d(weights, "weights")
+        w_ptr, w_pitch = weights.data_ptr(), _pitch(weights)
+    res = torch.empty(order.tokens, H, dtype=y.dtype, device=dev) if out is None else out
+    _call("b200moe_unpermute_rows", dev.index, y.data_ptr(), _DTYPE[y.dtype], _pitch(y), order._pointers[0], w_ptr, w_pitch,
+          order.tokens, order.top_k, H, res.data_ptr(), _pitch(res))
     return res
 
 
@@ -334,17 +349,15 @@ class _Unpermute(torch.autograd.Function):
         (rows, H), dtype = ctx.y_like
         dev = dout.device
         dout = _rows2d(dout, "grad")
-        dy = torch.empty((rows, H), dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty((order.tokens, order.top_k), dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
+        dy = torch.empty(rows, H, dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = torch.empty(order.tokens, order.top_k, dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
         y = None if dw is None else _rows2d(y, "y")
         w = None if weights is None else _rows2d(weights, "weights")
-        with _on(dev) as stream:
-            rc = _capi.lib().b200moe_unpermute_grad(
-                dout.data_ptr(), _DTYPE[dtype], _pitch(dout), None if y is None else y.data_ptr(), 0 if y is None else _pitch(y),
-                None if w is None else w.data_ptr(), 0 if w is None else _pitch(w), order.pos.data_ptr(), order.pair.data_ptr(),
-                order.offsets.data_ptr(), order.e_local, order.tokens, order.top_k, H, rows,
-                None if dy is None else dy.data_ptr(), H, None if dw is None else dw.data_ptr(), stream)
-        _capi.check(rc, "b200moe_unpermute_grad")
+        pos, pair, offsets = order._pointers
+        _call("b200moe_unpermute_grad", dev.index, dout.data_ptr(), _DTYPE[dtype], _pitch(dout),
+              None if y is None else y.data_ptr(), 0 if y is None else _pitch(y), None if w is None else w.data_ptr(),
+              0 if w is None else _pitch(w), pos, pair, offsets, order.e_local, order.tokens, order.top_k, H, rows,
+              None if dy is None else dy.data_ptr(), H, None if dw is None else dw.data_ptr())
         return dy, None, dw
 
 
@@ -356,7 +369,8 @@ def permute(x: torch.Tensor, order: TokenOrder, *, out: Optional[torch.Tensor] =
     (without ``out``): ``dx[t]`` is the sum of dy over the token's rows, in fp32, rounded once.
     """
     dev = _cuda(x, "x")
-    _same_device(dev, order=order.pos)
+    if order.device != dev:
+        raise _other_device(dev, order=order)
     if x.dim() != 2 or x.shape[0] != order.tokens:
         raise ValueError(f"x must be [{order.tokens}, H], got {tuple(x.shape)}")
     if x.element_size() not in (1, 2, 4) or x.is_complex():
@@ -381,7 +395,8 @@ def unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tensor
     pair takes are zero, dw is 0 where the expert is not local.
     """
     dev = _cuda(y, "y")
-    _same_device(dev, order=order.pos, weights=weights)
+    if order.device != dev or (weights is not None and weights.device != dev):
+        raise _other_device(dev, order=order, weights=weights)
     if y.dtype not in _DTYPE:
         raise TypeError(f"y must be float32, bfloat16 or float16, got {y.dtype}")
     if y.dim() != 2 or y.shape[0] != order.rows:

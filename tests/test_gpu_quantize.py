@@ -118,7 +118,7 @@ def test_special_values(dtype):
 @pytest.mark.parametrize("rows,cols", [(1, 2048), (67, 128), (5, 130), (33, 1), (64, 264)])
 def test_swiglu_form(dtype, rows, cols):
     """|code * scale - x| is half a step of e4m3 (2^-4 of the value, 2^-10 scales below its normal range) plus what fp32 makes of
-    the SwiGLU: the exponential is within 2 ulp, four more roundings of half an ulp, together below 2^-21."""
+    the SwiGLU: an exponential and a reciprocal within an ulp (2^-23 each), three roundings of half an ulp, below 2^-21 together."""
     g = torch.Generator().manual_seed(rows + cols)
     x = (4 * torch.randn(rows, 2 * cols, generator=g)).to(dtype)
     q, s = F.quantize(x.to(DEV), swiglu=True, scale_layout="tk")
@@ -130,6 +130,29 @@ def test_swiglu_form(dtype, rows, cols):
     se = s.cpu().double().repeat_interleave(128, 1)[:, :cols]
     err = (q.float().cpu().double() * se - ref).abs()
     assert (err <= torch.maximum(2.0 ** -4 * ref.abs(), 2.0 ** -10 * se) * (1 + 2.0 ** -20) + 2.0 ** -21 * ref.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_swiglu_special_values(dtype):
+    """Infinities, NaN and zeros go through g * (u * (1 / (1 + exp(-u)))) and the block as the formula says, from fp32 on."""
+    inf, nan = float("inf"), float("nan")
+    pairs = [(0.0, 0.0), (-0.0, 3.0), (1.0, inf), (1.0, -inf), (inf, 1.0), (-inf, 2.0), (0.0, inf), (nan, 1.0), (1.0, nan),
+             (2.0, -60000.0), (60000.0, 60000.0), (-60000.0, -3.0), (1.0, 100.0), (1.0, -100.0), (1e-7, 1e-7)]
+    x = torch.ones(len(pairs), 2 * 256, dtype=torch.float32)
+    for i, (g, u) in enumerate(pairs):
+        x[i, 5], x[i, 256 + 5] = g, u
+    x = x.to(dtype)
+    q, s = F.quantize(x.to(DEV), swiglu=True, scale_layout="tk")
+    f = x.float()
+    f = f[:, :256] * (f[:, 256:] * (1.0 / (1.0 + torch.exp(-f[:, 256:]))))
+    qr, sr = formula(f)
+    fin = sr.isfinite()
+    assert torch.equal(s.cpu()[~fin].nan_to_num(7.0), sr[~fin].nan_to_num(7.0))
+    assert ((s.cpu()[fin] - sr[fin]).abs() <= 2.0 ** -20 * sr[fin]).all()
+    qd, qrd = q.float().cpu(), qr.view(torch.float8_e4m3fn).float()
+    assert torch.equal(qd.isnan(), qrd.isnan())
+    # a quotient may take the neighbouring code: a step of e4m3 is at most 2^-3 of the value, 2^-9 below the normal range
+    assert ((qd - qrd).nan_to_num(0.0).abs() <= torch.maximum(2.0 ** -3 * qrd.abs().nan_to_num(0.0), torch.tensor(2.0 ** -9))).all()
 
 
 def test_refusals():

@@ -125,8 +125,7 @@ def test_row_moves_refusals(mem):
 def test_python_entry_points_refuse_cpu_tensors():
     x = torch.zeros(4, 256)
     ids = torch.zeros(4, 8, dtype=torch.int32)
-    table = torch.zeros(32, dtype=torch.int32)
-    order = F.TokenOrder(table[:17], table[:16], table.view(4, 8), table, 16, 0, 1)
+    order = F.TokenOrder(x.device, 4, 8, 32, 16, 0, 1)
     codes = torch.zeros(4, 256, dtype=torch.uint8)
     for call in (lambda: F.quantize(x), lambda: F.sort_tokens(ids), lambda: F.permute(x, order),
                  lambda: F.unpermute(torch.zeros(32, 256), order), lambda: F.block_matmul(codes, x, codes, x)):
