@@ -380,12 +380,14 @@ __device__ __forceinline__ void store_pack(P* p, const P& v) {
 
 constexpr int kSumBatch = 8;                     // rows of a token in flight together
 
-// A CTA takes one token's output row (or one of `segments` parts of it) after another: the rows' addresses are then known for the
-// whole row, eight loads a thread are in flight, and the next token's positions are on their way meanwhile.  (A warp for each
-// 512 bytes of an output row, which has to fetch the positions first, reached 3.5 TB/s of 14 KB rows, this 6.)
-template <typename T, int N, int U>
-__global__ void __launch_bounds__(kMoveThreads, 4)
-unpermute_kernel(const T* __restrict__ y, unsigned y_pitch, const int* __restrict__ pos, const float* __restrict__ weights,
+// A CTA takes a token's output row, or one of `segments` parts of it: the rows' addresses are then known for the whole row, and eight
+// loads a thread are in flight.  (A warp for each 512 bytes of an output row, which has to fetch the positions first, reached 3.5
+// TB/s of 14 KB rows, this 6.)  AHEAD: four CTAs an SM take one row after another, with the next one's positions on their way
+// meanwhile.  us, without / with: 8192 rows of 2048 bf16 62 / 53, 16384 of 512 69 / 49, 4096 of 7168 89 / 86; 4097 of 2048 fp32 47 /
+// 57, of 7168 153 / 184: fp32, whose sums take fewer registers, has six CTAs on an SM without it (with four of them 58 us).
+template <typename T, int N, int U, bool AHEAD>
+__global__ void __launch_bounds__(kMoveThreads, AHEAD ? 4 : 6)
+unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restrict__ pos, const float* __restrict__ weights,
                  long long w_stride, T* __restrict__ out, long long out_stride, int items, int top_k, int row_vecs,
                  int segments, int segment_vecs) {
   using P = Pack<T, N>;
@@ -401,23 +403,23 @@ unpermute_kernel(const T* __restrict__ y, unsigned y_pitch, const int* __restric
       w[j] = weights && k0 + j < top_k ? __ldg(weights + (size_t)t * w_stride + k0 + j) : 1.f;
     }
   };
-  int item = blockIdx.x;
-  if (item < items) fetch(item / segments, 0);
-  while (item < items) {
+  int item = blockIdx.x;                         // (below `items`)
+  fetch(item / segments, 0);
+  do {
     const int t = item / segments, v_begin = (item - t * segments) * segment_vecs, v_end = min(v_begin + segment_vecs, row_vecs);
     P* dst = reinterpret_cast<P*>(out + (size_t)t * out_stride);
-    int src[kSumBatch];
+    const P* src[kSumBatch];
     float weight[kSumBatch];
     auto use = [&] {
 #pragma unroll
       for (int j = 0; j < kSumBatch; ++j) {
-        src[j] = row[j];
+        src[j] = row[j] >= 0 ? reinterpret_cast<const P*>(y + row[j] * y_stride) : nullptr;
         weight[j] = w[j];
       }
     };
     use();
     item += gridDim.x;
-    if (top_k <= kSumBatch && item < items) fetch(item / segments, 0);
+    if (AHEAD && top_k <= kSumBatch && item < items) fetch(item / segments, 0);
     for (int v = v_begin + threadIdx.x; v < v_end; v += U * kMoveThreads) {
       float acc[U][N];
 #pragma unroll
@@ -428,17 +430,14 @@ unpermute_kernel(const T* __restrict__ y, unsigned y_pitch, const int* __restric
         P x[kSumBatch][U];
 #pragma unroll
         for (int j = 0; j < kSumBatch; ++j)
-          if (src[j] >= 0) {
-            // (one multiply-add: the pitch has 32 bits)
-            const P* at = reinterpret_cast<const P*>(reinterpret_cast<const uint8_t*>(reinterpret_cast<const P*>(y) + v) +
-                                                     (unsigned long long)(unsigned)src[j] * y_pitch);
+          if (src[j]) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
-              if (U == 1 || v + u * kMoveThreads < v_end) x[j][u] = load_pack(at + u * kMoveThreads);
+              if (U == 1 || v + u * kMoveThreads < v_end) x[j][u] = load_pack(src[j] + v + u * kMoveThreads);
           }
 #pragma unroll
         for (int j = 0; j < kSumBatch; ++j)
-          if (src[j] >= 0) {
+          if (src[j]) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -458,8 +457,8 @@ unpermute_kernel(const T* __restrict__ y, unsigned y_pitch, const int* __restric
         if (U == 1 || v + u * kMoveThreads < v_end) store_pack(dst + v + u * kMoveThreads, r);
       }
     }
-    if (top_k > kSumBatch && item < items) fetch(item / segments, 0);
-  }
+    if (AHEAD && top_k > kSumBatch && item < items) fetch(item / segments, 0);
+  } while (AHEAD && item < items);
 }
 
 template <typename T>
@@ -566,22 +565,18 @@ template <typename T, int N>
 cudaError_t launch_unpermute(const void* y, long long y_stride, const int* pos, const float* weights, long long w_stride, void* out,
                              long long out_stride, int tokens, int top_k, int hidden, int num_sms, cudaStream_t stream) {
   constexpr int U = sizeof(T) * N == 16 ? 1 : sizeof(T) * N == 4 ? 2 : 4;   // loads of fewer bytes: more of them in flight
-  static const int resident = [] {                // CTAs on an SM: 4 to 6, by the registers that a type takes
-    int n = 0;
-    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, unpermute_kernel<T, N, U>, kMoveThreads, 0) == cudaSuccess && n > 0 ? n : 4;
-  }();
   const int row_vecs = hidden / N;
   // one CTA a token, more where that leaves SMs without one
   const int pieces = (row_vecs + kMoveThreads - 1) / kMoveThreads;
-  const long long ctas = (long long)resident * num_sms;
-  int segments = (int)((ctas + tokens - 1) / tokens);
+  constexpr bool kAhead = sizeof(T) == 2;
+  int segments = (int)(((kAhead ? 4ll : 8ll) * num_sms + tokens - 1) / tokens);
   if (segments > pieces) segments = pieces;
   const int segment_vecs = (pieces + segments - 1) / segments * kMoveThreads;
   segments = (row_vecs + segment_vecs - 1) / segment_vecs;
   const long long items = (long long)tokens * segments;
-  if (items > 0x7fffffffll - ctas) return cudaErrorInvalidValue;   // (a token in parts: few tokens)
-  return launch_chained(unpermute_kernel<T, N, U>, dim3(grid_for(items, ctas)), dim3(kMoveThreads), 0, stream,
-                        reinterpret_cast<const T*>(y), (unsigned)(y_stride * sizeof(T)), pos, weights, w_stride, reinterpret_cast<T*>(out), out_stride,
+  if (items > 0x7fffffffll - 8ll * num_sms) return cudaErrorInvalidValue;   // (a token in parts: few tokens)
+  return launch_chained(unpermute_kernel<T, N, U, kAhead>, dim3(grid_for(items, kAhead ? 4ll * num_sms : items)), dim3(kMoveThreads), 0, stream,
+                        reinterpret_cast<const T*>(y), y_stride, pos, weights, w_stride, reinterpret_cast<T*>(out), out_stride,
                         (int)items, top_k, row_vecs, segments, segment_vecs);
 }
 
@@ -777,7 +772,6 @@ int b200moe_unpermute_rows(const void* y, int dtype, int64_t y_row_stride, const
     return B200MOE_ERR_INVALID_ARGUMENT;
   const uintptr_t size = dtype == B200MOE_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(y) % size != 0 || reinterpret_cast<uintptr_t>(out) % size != 0) return B200MOE_ERR_MISALIGNED;
-  if (y_row_stride > (int64_t)(0xffffffffu / size)) return B200MOE_ERR_UNSUPPORTED_SHAPE;   // a pitch of 32 bits
   int num_sms = 0;
   if ((rc = ensure_device(&num_sms)) != B200MOE_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
