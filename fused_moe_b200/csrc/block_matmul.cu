@@ -8,6 +8,12 @@
 //
 // Two kernels: 128 x 128 tiles, two CTAs on an SM, the K blocks of a tile divided over a cluster where tiles are few; and
 // 256 x 256 tiles of a CTA pair (cta_group::2) where there are enough of them.
+//
+// Few rows are bound by the weights' bytes and, below some 30 MB of them, by latency: one row through 4096 x 7168 takes 8.8 us (29
+// MB, 4.5 us at the copy rate), through 7168 x 16384 23.9 us (117 MB, 17.9).  Many rows are bound by the hand-offs between tensor
+// cores and promotion: 8192 x 4096 x 7168 takes 229 us, 2.1 PFLOP/s, some 1000 cycles for a K block of a tile whose MMAs take 512.
+// An accumulator's way round - issue 200 cycles, MMAs 260 to 510, the look at the barrier 200 to 300, read-back 250 to 300, the
+// counter's way back 200 and more - is longer than the MMAs of the other one, and tensor memory has no room for a third.
 #include "common.cuh"
 #include "host.cuh"
 #include "kernels.cuh"
@@ -118,9 +124,9 @@ __device__ __forceinline__ void fold(float2* acc, const uint32_t (&r)[32], float
     acc[j] = __ffma2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[j]);
 }
 
-// Folds one K block's 128 columns of a TMEM lane into `acc`; `release`, which hands the
-// accumulator back, runs once the last of them sits in registers.  `look` looks at the next K block's barriers without waiting:
-// where the tensor cores are ahead its answer, some 200 cycles later, costs nothing.
+// Folds one K block's 128 columns of a TMEM lane into `acc`; `release`, which hands the accumulator back, runs once the last of
+// them sits in registers.  `look` looks at the next K block's barriers without waiting: where the tensor cores are ahead its
+// answer, some 200 cycles later, costs nothing.
 template <typename Look, typename Release>
 __device__ __forceinline__ void promote(float2* acc, uint32_t taddr, float s, Look look, Release release) {
   uint32_t ra[32], rb[32];
@@ -193,7 +199,6 @@ __device__ __forceinline__ float ld_factor(uint32_t addr) {
 // "These TMEM columns sit in my registers", added to a counter (and, for a factor slot, to a barrier) at a shared::cluster
 // address.  Relaxed: what it publishes was completed by tcgen05.wait::ld, the tcgen05 fences on both sides order the tensor-memory
 // accesses; a releasing arrival waits for the thread's loads from global memory first (1000 cycles a K block, when it had some).
-// The issuer polls the counter with plain loads, a fifth of what a look at a barrier takes.
 __device__ __forceinline__ void count_relaxed(uint32_t cluster_addr) {
   asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], 1;" ::"r"(cluster_addr) : "memory");
 }
@@ -266,13 +271,13 @@ static_assert(128 * (kMidLaunchRegs - kMidCtrlRegs) >= 128 * (kMidPromoRegs - kM
 template <int S>
 __device__ __forceinline__ void join_split(const MatmulParams& p, const float2* acc, uint32_t smem_base, int thread, int rows, int m0,
                                            int n0) {
-  constexpr int most = (kTile / 4 + S - 1) / S;   // vectors of a part
+  constexpr int kMost = (kTile / 4 + S - 1) / S;   // vectors of a part
   const int me = S > 1 ? (int)cluster_rank() : 0;
   if (thread < rows) {
 #pragma unroll
     for (int c = 0; c < kTile / 4; ++c) {
       const int j = ((c + 1) * S - 1) / (kTile / 4);   // the CTA whose part [32 j / S, 32 (j + 1) / S) has c
-      const uint32_t at = smem_base + ((me * most + c - kTile / 4 * j / S) * kTile + thread) * 16;
+      const uint32_t at = smem_base + ((me * kMost + c - kTile / 4 * j / S) * kTile + thread) * 16;
       const float2 x = acc[2 * c], y = acc[2 * c + 1];
       if (S > 1) st_cluster_v4(map_to_rank(at, (uint32_t)j), x.x, x.y, y.x, y.y);
       else st_shared_v4(at, x.x, x.y, y.x, y.y);
@@ -294,7 +299,7 @@ __device__ __forceinline__ void join_split(const MatmulParams& p, const float2* 
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     float4 v[S];
 #pragma unroll
-    for (int j = 0; j < S; ++j) v[j] = ld_shared_v4(smem_base + ((j * most + c) * kTile + row) * 16);
+    for (int j = 0; j < S; ++j) v[j] = ld_shared_v4(smem_base + ((j * kMost + c) * kTile + row) * 16);
 #pragma unroll
     for (int j = 0; j < S; ++j) {
       sum.x += v[j].x;

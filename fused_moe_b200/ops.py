@@ -14,7 +14,9 @@ The layer from parts is the sequence route, sort_tokens, permute, quantize, bloc
 block_matmul, unpermute.  All results repeat bit for bit (there are no atomics on values), every call is asynchronous on the
 current stream of its tensors' device, can be captured into a CUDA graph and allocates only its results (and the sort, above
 16384 pairs, a scratch tensor) from torch's allocator.  Errors: ``TypeError`` / ``ValueError`` for arguments, ``RuntimeError``
-for tensors that are not on one CUDA device, ``MoEError`` for what the library refuses.
+for tensors that are not on one CUDA device, ``MoEError`` for what the library refuses.  A backward pass is captured like any of
+torch's: after a warm-up on a side stream, with no earlier graph of the same leaves alive (torch warns about its AccumulateGrad
+node and the capture fails).  Gradients are first order.
 
 The reference has no counterparts: its only public function is the fused layer (solution/python/kernel.py:642-648).
 """

@@ -152,3 +152,38 @@ def test_a_training_step_with_experts_between_captured_too():
     for a, b in zip(captured, eager):
         assert torch.equal(a, b)
     assert torch.equal(step()[0], eager[0])
+
+
+def test_offsets_beyond_32_bits():
+    """Rows behind the 4 GiB mark of every operator's large side, spot-checked where the offset has more than 32 bits."""
+    T, H, K = 40960, 7168, 8                         # sorted rows: 4.7 GB of bf16
+    ids = torch.arange(T * K, device=DEV).view(T, K) % 16
+    order = F.sort_tokens(ids, 16)
+    x = torch.arange(T, device=DEV, dtype=torch.float32)[:, None].expand(T, H).bfloat16().contiguous()
+    rows = F.permute(x, order)
+    tail = order.pair[-1000:].long() // K
+    assert torch.equal(rows[-1000:], x[tail])
+    out = F.unpermute(rows, order, torch.full((T, K), 0.125, device=DEV))
+    assert torch.equal(out, x)
+    del out
+    y = rows.requires_grad_(True)
+    dy, = torch.autograd.grad(F.unpermute(y, order), y, x)
+    assert torch.equal(dy[-1000:], x[tail])
+    del rows, y, dy
+    big = torch.zeros(T, 65536, device=DEV, dtype=torch.bfloat16)    # 5.4 GB of activations, 2.7 GB of codes
+    big[-1] = torch.randn(65536, device=DEV)
+    q, s = F.quantize(big)
+    one, so = F.quantize(big[-1:])
+    assert torch.equal(q[-1:].view(torch.uint8), one.view(torch.uint8)) and torch.equal(s[:, -1:], so)
+    assert not q[:-1].view(torch.uint8).any()
+    del big
+    w = torch.zeros(128, 65536, device=DEV, dtype=torch.uint8)
+    w[:, ::512] = 0x38                                               # ones
+    sw = torch.ones(1, 512, device=DEV)
+    small = F.block_matmul(one, so, w, sw, out_dtype=torch.float32)
+    wide = torch.empty(T, 32768, device=DEV, dtype=torch.float32)    # 5.4 GB, of which the first 128 columns are the result
+    F.block_matmul(q, s, w, sw, out=wide[:, :128])
+    ref = (one.double() * so.double().t().repeat_interleave(128, 1))[:, ::512].sum()
+    for got in (small[0], wide[-1, :128]):
+        assert ((got.double() - ref).abs() <= 2.0 ** -13 * (one.double().abs() * so.double().t().repeat_interleave(128, 1))[:, ::512].sum()).all()
+    assert not wide[:-1, :128].any()
