@@ -124,15 +124,14 @@ __device__ __forceinline__ void fold(float2* acc, const uint32_t (&r)[32], float
     acc[j] = __ffma2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[j]);
 }
 
-// Folds one K block's 128 columns of a TMEM lane into `acc`; `release`, which hands the accumulator back, runs once the last of
-// them sits in registers.  `look` looks at the next K block's barriers without waiting: where the tensor cores are ahead its
-// answer, some 200 cycles later, costs nothing.
-template <typename Look, typename Release>
-__device__ __forceinline__ void promote(float2* acc, uint32_t taddr, float s, Look look, Release release) {
+// Folds one K block's 128 columns of a TMEM lane into `acc`; `release` runs once the last of them sits in registers: it hands the
+// accumulator back and looks at the next K block's barriers without waiting, so that the last FMAs cover the look's latency.  (A
+// look already at the first read-back, where it mostly comes too early, took 2 % more time.)
+template <typename Release>
+__device__ __forceinline__ void promote(float2* acc, uint32_t taddr, float s, Release release) {
   uint32_t ra[32], rb[32];
   tmem_ld_32x32(taddr, ra);
   tmem_ld_32x32(taddr + 32, rb);
-  look();
   tmem_ld_wait_on(ra, rb);
   fold(acc, ra, s);
   tmem_ld_32x32(taddr + 64, ra);
@@ -434,17 +433,14 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
       }
       tc_fence_after();
       const float f = ld_factor(factors + ((it % kScaleRing) * kTile + threadIdx.x - 128) * 4);
-      const auto look = [&] {
-        const uint32_t n = it + 1;
-        seen_f = mbar_test_wait(bar_factors + 8 * (n % kScaleRing), (n / kScaleRing) & 1);
-        seen_d = mbar_test_wait(bar_done + 8 * (n % kMidAcc), (n / kMidAcc) & 1);
-      };
-      promote(acc, tmem + ((uint32_t)((warp - 4) * 32) << 16) + b * kTile, f, look, [&] {
+      promote(acc, tmem + ((uint32_t)((warp - 4) * 32) << 16) + b * kTile, f, [&] {
         if (lane == 0) {
           count_relaxed(own + count_read + 4 * b);
           mbar_arrive_relaxed(own + bar_slot + 8 * (it % kScaleRing));
         }
-        if (!seen_d) seen_d = mbar_test_wait(bar_done + 8 * ((it + 1) % kMidAcc), ((it + 1) / kMidAcc) & 1);
+        const uint32_t n = it + 1;
+        seen_f = mbar_test_wait(bar_factors + 8 * (n % kScaleRing), (n / kScaleRing) & 1);
+        seen_d = mbar_test_wait(bar_done + 8 * (n % kMidAcc), (n / kMidAcc) & 1);
       });
       seen_f = __all_sync(0xffffffffu, seen_f);
       seen_d = __all_sync(0xffffffffu, seen_d);
@@ -700,17 +696,14 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
         }
         tc_fence_after();
         const float f = ld_factor(factors + ((it % kScaleRing) * 2 * kTile + threadIdx.x - 128) * 4);
-        const auto look = [&] {
-          const uint32_t n = it + 1;
-          seen_f = mbar_test_wait(bar_factors + 8 * (n % kScaleRing), (n / kScaleRing) & 1);
-          seen_d = mbar_test_wait(bar_done + 8 * (2 * half + (n & 1)), (n >> 1) & 1);
-        };
-        promote(acc, taddr + b * kTile, f, look, [&] {
+        promote(acc, taddr + b * kTile, f, [&] {
           if (lane == 0) {
             count_relaxed(read + 4 * b);
             mbar_arrive_relaxed(slot + 8 * (it % kScaleRing));
           }
-          if (!seen_d) seen_d = mbar_test_wait(bar_done + 8 * (2 * half + ((it + 1) & 1)), ((it + 1) >> 1) & 1);
+          const uint32_t n = it + 1;
+          seen_f = mbar_test_wait(bar_factors + 8 * (n % kScaleRing), (n / kScaleRing) & 1);
+          seen_d = mbar_test_wait(bar_done + 8 * (2 * half + (n & 1)), (n >> 1) & 1);
         });
         seen_f = __all_sync(0xffffffffu, seen_f);
         seen_d = __all_sync(0xffffffffu, seen_d);
@@ -763,7 +756,8 @@ long long mid_cost(long long tiles, int kblocks, int rows, int S, int num_sms) {
   const long long steps = (kblocks + S - 1) / S;
   const long long one = steps * 360 + (S == 1 ? 300 : 400 + rows * (2300 + 250 * S) / kTile);
   const long long two = steps * 590 + (S == 1 ? 300 : 600 + rows * (800 + 1000 * S) / kTile);
-  return full * two + (rest == 0 ? 0 : rest <= (S == 1 ? num_sms : num_sms * 7 / 8) ? one : two);
+  // (from the third wave on L2 has 13 TB/s to deliver)
+  return (full >= 2 ? full * two * 9 / 8 : full * two) + (rest == 0 ? 0 : rest <= (S == 1 ? num_sms : num_sms * 7 / 8) ? one : two);
 }
 // 256 x 256 tiles, one pair of SMs each.  M x 1536 x 7168, 128 x 128 tiles / pairs: M 1536 23.1 / 31.0, 2048 32.9 / 32.3, 4096 54.6 /
 // 59.5; M x 4096 x 7168: 640 32.7 / 32.8, 1024 33.3 / 32.0, 1536 54.8 / 59.7, 2048 65.8 / 59.7, 3000 104.7 / 88.5, 8192 274 / 228;
