@@ -31,6 +31,7 @@ from . import _capi
 from ._capi import MoEError
 from .kernel import BLOCK, E_GLOBAL
 
+_INT_MAX = 2 ** 31 - 1
 _SORT_ONE_LAUNCH = 16384      # pairs that the sort handles without a scratch tensor
 _CODES = (torch.float8_e4m3fn, torch.uint8)
 _DTYPE = {torch.float32: _capi.F32, torch.bfloat16: _capi.BF16, torch.float16: _capi.F16}
@@ -41,9 +42,14 @@ _current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+_functions: Dict[str, object] = {}
+
+
 def _call(name: str, index: int, *args) -> None:
     """Library call with its device current, on that device's current stream (the last argument)."""
-    fn = getattr(_capi.lib(), name)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_capi.lib(), name)
     if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
@@ -53,10 +59,8 @@ def _call(name: str, index: int, *args) -> None:
         _capi.check(rc, name)
 
 
-def _cuda(t: torch.Tensor, what: str) -> torch.device:
-    if not t.is_cuda:
-        raise RuntimeError(f"{what} is on {t.device}: fused_moe_b200 runs on CUDA tensors only (there is no CPU path)")
-    return t.device
+def _not_cuda(t: torch.Tensor, what: str) -> RuntimeError:
+    return RuntimeError(f"{what} is on {t.device}: fused_moe_b200 runs on CUDA tensors only (there is no CPU path)")
 
 
 def _other_device(dev: torch.device, **tensors) -> RuntimeError:
@@ -65,17 +69,16 @@ def _other_device(dev: torch.device, **tensors) -> RuntimeError:
     return RuntimeError(f"{name} is on {t.device}, the other arguments on {dev}")
 
 
-def _no_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
+def _no_gradient(what: str) -> RuntimeError:
+    return RuntimeError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
 def _rows2d(t: torch.Tensor, what: str) -> torch.Tensor:
-    """``t`` with unit inner stride and rows that do not overlap (a copy where it has not)."""
+    """``t`` with unit inner stride and rows that do not overlap (a copy where it has not); extents that 32 bits hold."""
     if t.dim() != 2:
         raise ValueError(f"{what} must be 2-D, got shape {tuple(t.shape)}")
+    if t.shape[0] > _INT_MAX or t.shape[1] > _INT_MAX:
+        raise ValueError(f"{what} must have at most {_INT_MAX} rows and columns, got shape {tuple(t.shape)}")
     if t.is_contiguous():
         return t
     if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
@@ -107,13 +110,16 @@ def quantize(x: torch.Tensor, *, swiglu: bool = False, scale_layout: str = "kt")
     [T, ceil(K/128)].  With ``swiglu`` the input is [T, 2K] and what is quantised is ``x[:, :K] * silu(x[:, K:])`` in fp32.
     A block that holds an infinity or a NaN gets it as its scale, and codes as the quotient says.  Any K; not differentiable.
     """
-    dev = _cuda(x, "x")
+    if not x.is_cuda:
+        raise _not_cuda(x, "x")
+    dev = x.device
     dt = _DTYPE.get(x.dtype)
     if dt is None:
         raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
     if scale_layout not in ("kt", "tk"):
         raise ValueError(f"scale_layout must be 'kt' or 'tk', got {scale_layout!r}")
-    _no_grad("quantize", x)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise _no_gradient("quantize")
     x = _rows2d(x, "x")
     rows, cols = x.shape
     if swiglu:
@@ -175,18 +181,22 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     must have unit inner stride and such a pitch.  Scales may have any strides.  ``out`` writes into a tensor of the caller's
     (which must not overlap the inputs).  Not differentiable: the operands are codes.
     """
-    dev = _cuda(a, "a")
+    if not a.is_cuda:
+        raise _not_cuda(a, "a")
+    dev = a.device
     if a_scale.device != dev or b.device != dev or b_scale.device != dev:
         raise _other_device(dev, a_scale=a_scale, b=b, b_scale=b_scale)
-    _no_grad("block_matmul", a_scale, b_scale)
-    for name, t in (("a", a), ("b", b)):
-        if t.dtype not in _CODES:
-            raise TypeError(f"{name} must be float8_e4m3fn (or its uint8 bit pattern), got {t.dtype}")
+    if (a_scale.requires_grad or b_scale.requires_grad) and torch.is_grad_enabled():
+        raise _no_gradient("block_matmul")
+    if a.dtype not in _CODES or b.dtype not in _CODES:
+        raise TypeError(f"a and b must be float8_e4m3fn (or its uint8 bit pattern), got {a.dtype} and {b.dtype}")
     a = _rows2d(a, "a")
     M, K = a.shape
     if b.dim() != 2 or b.shape[1] != K:
         raise ValueError(f"b must be [N, {K}], got {tuple(b.shape)}")
     N = b.shape[0]
+    if N > _INT_MAX:
+        raise ValueError(f"b must have at most {_INT_MAX} rows, got {N}")
     if K == 0 or K % 16:
         raise ValueError(f"K must be a positive multiple of 16, got {K}")
     if scale_layout not in ("kt", "tk"):
@@ -273,7 +283,9 @@ def sort_tokens(topk_ids: torch.Tensor, e_local: int = E_GLOBAL, local_expert_of
     expert that a token names twice gets two.  Each expert's rows start on a multiple of ``align`` (128: a matrix tile).  The
     order has ``T * top_k`` rows and, with ``align``, room for the padding: how many are in use stays on the device.
     """
-    dev = _cuda(topk_ids, "topk_ids")
+    if not topk_ids.is_cuda:
+        raise _not_cuda(topk_ids, "topk_ids")
+    dev = topk_ids.device
     if topk_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
     ids = _rows2d(topk_ids, "topk_ids")
@@ -370,7 +382,9 @@ def permute(x: torch.Tensor, order: TokenOrder, *, out: Optional[torch.Tensor] =
     zero too, except in an ``out`` of the caller's, where they stay as they were.  Differentiable for fp32, bf16 and fp16 x
     (without ``out``): ``dx[t]`` is the sum of dy over the token's rows, in fp32, rounded once.
     """
-    dev = _cuda(x, "x")
+    if not x.is_cuda:
+        raise _not_cuda(x, "x")
+    dev = x.device
     if order.device != dev:
         raise _other_device(dev, order=order)
     if x.dim() != 2 or x.shape[0] != order.tokens:
@@ -396,7 +410,9 @@ def unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tensor
     token without any is zero) whatever their weight.  Differentiable in y and weights (without ``out``): rows of dy that no
     pair takes are zero, dw is 0 where the expert is not local.
     """
-    dev = _cuda(y, "y")
+    if not y.is_cuda:
+        raise _not_cuda(y, "y")
+    dev = y.device
     if order.device != dev or (weights is not None and weights.device != dev):
         raise _other_device(dev, order=order, weights=weights)
     if y.dtype not in _DTYPE:
