@@ -155,6 +155,21 @@ def test_swiglu_special_values(dtype):
     assert ((qd - qrd).nan_to_num(0.0).abs() <= torch.maximum(2.0 ** -3 * qrd.abs().nan_to_num(0.0), torch.tensor(2.0 ** -9))).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_swiglu_far_down(dtype):
+    """1 + exp(-u) up to where the exponential overflows, whose reciprocal is below fp32's normal range, times large numbers: the
+    scale within 2^-21 of the formula's (see test_swiglu_form) and half an ulp, 2^-24, of the division."""
+    u = torch.tensor([-86.5, -87.0, -87.5, -88.0, -88.5, -40.0, -3.0]).to(dtype)
+    x = torch.zeros(len(u), 256)
+    x[:, 7], x[:, 128 + 7] = 1e37, u.float()
+    x = x.to(dtype)
+    q, s = F.quantize(x.to(DEV), swiglu=True, scale_layout="tk")
+    d = x.double()
+    ref = (d[:, 7] * d[:, 128 + 7] * torch.sigmoid(d[:, 128 + 7])).abs() / 448
+    assert ((s.cpu()[:, 0].double() - ref).abs() <= ref * (2.0 ** -21 + 2.0 ** -23)).all()
+    assert (q.float().cpu()[:, 7] == -448).all()
+
+
 def test_refusals():
     x = torch.zeros(4, 256, device=DEV)
     with pytest.raises(TypeError):
