@@ -22,7 +22,8 @@ constexpr int kMaxSortTopK = 32;                 // a token's positions are held
 constexpr int kSortWarps = 16;
 constexpr int kSortThreads = 32 * kSortWarps;
 constexpr int kSortCluster = 8;                  // CTAs that one launch sorts with
-constexpr int kSortRounds = 4, kSortManyRounds = 16;   // pairs of a thread
+constexpr int kSortRounds = 4;                   // pairs of a thread
+constexpr int kSortChunk = kSortThreads * kSortRounds;
 
 struct SortParams {
   const void* ids;
@@ -39,6 +40,7 @@ struct SortParams {
   int* pair;                                     // [rows]
   int* chunk_counts;                             // [chunks][e_local] of the kernel before; null: the chunks are one cluster
   int chunks;
+  int scanned;                                   // chunk_counts [chunks + 1][e_local] holds the sums over the chunks before
 };
 
 __device__ __forceinline__ int local_expert(const SortParams& p, int i) {
@@ -51,34 +53,69 @@ __device__ __forceinline__ int local_expert(const SortParams& p, int i) {
   return id >= p.local_off && id < (long long)p.local_off + p.e_local ? (int)(id - p.local_off) : -1;
 }
 
-// Expert of each of a thread's R pairs (-1: not local, or past the end): warp w of chunk c has pairs
-// [(c * kSortWarps + w) * 32 R, + 32 R), round r its 32 from 32 r on.  All loads are in flight together.
-template <int R>
-__device__ __forceinline__ long long load_experts(const SortParams& p, int (&e)[R]) {
-  const long long first = ((long long)blockIdx.x * kSortWarps + (threadIdx.x >> 5)) * (32 * R) + (threadIdx.x & 31);
+// Expert of each of a thread's pairs (-1: not local, or past the end): warp w of chunk c has the 32 x kSortRounds pairs from
+// (c * kSortWarps + w) * 32 kSortRounds on, round r 32 of them.  All loads are in flight together.
+__device__ __forceinline__ long long load_experts(const SortParams& p, int (&e)[kSortRounds]) {
+  const long long first = ((long long)blockIdx.x * kSortWarps + (threadIdx.x >> 5)) * (32 * kSortRounds) + (threadIdx.x & 31);
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
+  for (int r = 0; r < kSortRounds; ++r) {
     const long long i = first + r * 32;
     e[r] = i < p.pairs ? local_expert(p, (int)i) : -1;
   }
   return first;
 }
 
-template <int R>
 __global__ void __launch_bounds__(kSortThreads)
 sort_count_kernel(const __grid_constant__ SortParams p) {
   extern __shared__ int s_cnt[];                 // [e_local]
   for (int e = threadIdx.x; e < p.e_local; e += kSortThreads) s_cnt[e] = 0;
   chain_wait();
   chain_release();
-  int e[R];
-  load_experts<R>(p, e);
+  int e[kSortRounds];
+  load_experts(p, e);
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int r = 0; r < kSortRounds; ++r)
     if (e[r] >= 0) atomicAdd(s_cnt + e[r], 1);
   __syncthreads();
   for (int x = threadIdx.x; x < p.e_local; x += kSortThreads) p.chunk_counts[(size_t)blockIdx.x * p.e_local + x] = s_cnt[x];
+}
+
+// The counts of many chunks become the sums over the chunks before, with the totals behind them: a warp takes 32 experts'
+// neighbouring counters through a 32nd of the chunks, first for its sum and then for the sums before each chunk.
+__global__ void __launch_bounds__(1024)
+sort_scan_kernel(const __grid_constant__ SortParams p) {
+  __shared__ int s_sum[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = p.e_local, x = (int)blockIdx.x * 32 + lane;
+  const int per = (p.chunks + 31) / 32, c0 = warp * per, c1 = min(c0 + per, p.chunks);
+  chain_wait();
+  chain_release();
+  int sum = 0;
+  if (x < E) {
+#pragma unroll 16
+    for (int c = c0; c < c1; ++c) sum += p.chunk_counts[(size_t)c * E + x];
+  }
+  s_sum[warp][lane] = sum;
+  __syncthreads();
+  if (x >= E) return;
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 32; ++w) {
+    const int n = s_sum[w][lane];
+    before += w < warp ? n : 0;
+    total += n;
+  }
+  for (int c = c0; c < c1; c += 16) {
+    int n[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) n[j] = c + j < c1 ? p.chunk_counts[(size_t)(c + j) * E + x] : 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (c + j < c1) p.chunk_counts[(size_t)(c + j) * E + x] = before;
+      before += n[j];
+    }
+  }
+  if (warp == 0) p.chunk_counts[(size_t)p.chunks * E + x] = total;
 }
 
 // Exclusive sum over the CTA's threads.
@@ -113,7 +150,6 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
 // pairs of the same expert is the counter plus its rank in a match of the expert over the warp, a warp's first place the sum over
 // the warps before it.  What the other chunks hold comes out of their shared memory (the chunks are one cluster: one launch),
 // or out of the kernel before.  What this takes is latency: no loop over anything but rounds, warps and chunks.
-template <int R>
 __global__ void __launch_bounds__(kSortThreads)
 sort_place_kernel(const __grid_constant__ SortParams p) {
   extern __shared__ __align__(16) int smem[];
@@ -128,12 +164,12 @@ sort_place_kernel(const __grid_constant__ SortParams p) {
   for (int i = threadIdx.x; i < (kSortWarps + 2) * E; i += kSortThreads) smem[i] = 0;
   chain_wait();
   chain_release();
-  int e[R], rank[R];
-  const long long first_pair = load_experts<R>(p, e);
+  int e[kSortRounds], rank[kSortRounds];
+  const long long first_pair = load_experts(p, e);
   __syncthreads();
   int* mine = s_cnt + warp * E;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
+  for (int r = 0; r < kSortRounds; ++r) {
     const unsigned same = __match_any_sync(0xffffffffu, e[r]);
     const int before = e[r] >= 0 ? mine[e[r]] : 0;
     rank[r] = before + __popc(same & ((1u << lane) - 1u));
@@ -174,6 +210,11 @@ sort_place_kernel(const __grid_constant__ SortParams p) {
     }
     __syncwarp();
     cluster_arrive();                            // waited for at the end: peers may still read this CTA's counts
+  } else if (p.scanned) {
+    for (int x = threadIdx.x; x < E; x += kSortThreads) {
+      s_total[x] = p.chunk_counts[(size_t)p.chunks * E + x];
+      s_before[x] = p.chunk_counts[(size_t)blockIdx.x * E + x];
+    }
   } else if (p.chunk_counts) {
     const int parts = E < kSortThreads ? kSortThreads / E : 1;
     const int per = (p.chunks + parts - 1) / parts;
@@ -220,7 +261,7 @@ sort_place_kernel(const __grid_constant__ SortParams p) {
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
+  for (int r = 0; r < kSortRounds; ++r) {
     const long long i = first_pair + r * 32;
     const int row = e[r] >= 0 ? s_first[e[r]] + s_before[e[r]] + mine[e[r]] + rank[r] : -1;
     if (i < p.pairs) p.pos[i] = row;
@@ -244,18 +285,16 @@ sort_place_kernel(const __grid_constant__ SortParams p) {
 
 size_t sort_place_smem(int e_local) { return ((size_t)(kSortWarps + 4) * e_local + 1) * 4; }
 
-// How a number of pairs is sorted: chunks of 512 x `rounds` pairs, in one launch (of one cluster) or in two.
+// How a number of pairs is sorted: chunks of kSortChunk pairs, in one launch (of one cluster) or in two.  (Four times as many pairs
+// a thread took longer at every size: 28 us instead of 19 for 2^19 pairs of 256 experts.)
 struct SortPlan {
-  int rounds, chunks;
+  int chunks;
   bool one_launch;
 };
 SortPlan sort_plan(long long pairs, long long rows) {
-  constexpr int kSmall = kSortThreads * kSortRounds, kLarge = kSortThreads * kSortManyRounds;
   SortPlan s;
-  s.one_launch = pairs <= (long long)kSortCluster * kSmall;
-  s.rounds = pairs <= 256ll * kSmall ? kSortRounds : kSortManyRounds;
-  const int chunk = s.rounds == kSortRounds ? kSmall : kLarge;
-  s.chunks = pairs > 0 ? (int)((pairs + chunk - 1) / chunk) : 1;
+  s.one_launch = pairs <= (long long)kSortCluster * kSortChunk;
+  s.chunks = pairs > 0 ? (int)((pairs + kSortChunk - 1) / kSortChunk) : 1;
   if (s.one_launch) {
     // clusters of 1, 2, 4, 8; CTAs without pairs where many empty rows are to be marked (16 tokens of 256 experts whose segments
     // start on multiples of 128: 32640 rows)
@@ -264,14 +303,18 @@ SortPlan sort_plan(long long pairs, long long rows) {
   }
   return s;
 }
+// Every chunk adds up what the others have of each expert, which goes with the square of the chunks; from this many counters
+// on a launch of its own makes running sums of them.  us without / with (experts x chunks): 8 x 256 9.0 / 12.6; 256 x 64 10.0 /
+// 12.1, x 128 17.3 / 13.2, x 1024 72 / 47; 1024 x 32 12.6 / 12.8, x 64 15.8 / 13.2, x 256 52.6 / 19.9.
+constexpr long long kSortScanCounters = 24576;
 
-template <int R>
 cudaError_t launch_sort(const SortParams& p, const SortPlan& plan, cudaStream_t stream) {
   if (!plan.one_launch) {
-    const cudaError_t e = launch_chained(sort_count_kernel<R>, dim3(plan.chunks), dim3(kSortThreads), (size_t)p.e_local * 4, stream, p);
+    cudaError_t e = launch_chained(sort_count_kernel, dim3(plan.chunks), dim3(kSortThreads), (size_t)p.e_local * 4, stream, p);
+    if (e == cudaSuccess && p.scanned) e = launch_chained(sort_scan_kernel, dim3((p.e_local + 31) / 32), dim3(1024), 0, stream, p);
     if (e != cudaSuccess) return e;
   }
-  return launch_chained_cluster(sort_place_kernel<R>, dim3(plan.chunks), dim3(kSortThreads), sort_place_smem(p.e_local), stream,
+  return launch_chained_cluster(sort_place_kernel, dim3(plan.chunks), dim3(kSortThreads), sort_place_smem(p.e_local), stream,
                                 plan.one_launch ? plan.chunks : 1, p);
 }
 
@@ -647,10 +690,7 @@ int order_ok(int64_t tokens, int top_k, int64_t rows) {
 }  // namespace
 
 cudaError_t configure_sort_rows() {
-  const int bytes = (int)sort_place_smem(kMaxSortExperts);
-  const cudaError_t e = cudaFuncSetAttribute(sort_place_kernel<kSortRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(sort_place_kernel<kSortManyRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sort_place_smem(kMaxSortExperts));
 }
 
 }  // namespace b200moe
@@ -670,7 +710,7 @@ int64_t b200moe_sort_rows(int64_t tokens, int top_k, int e_local, int align) {
 int64_t b200moe_sort_workspace_bytes(int64_t tokens, int top_k, int e_local) {
   if (order_ok(tokens, top_k, 0) != B200MOE_OK || e_local < 1 || e_local > kMaxSortExperts) return B200MOE_ERR_INVALID_ARGUMENT;
   const SortPlan plan = sort_plan(tokens * top_k, 0);
-  return plan.one_launch ? 0 : (int64_t)plan.chunks * e_local * 4;
+  return plan.one_launch ? 0 : (int64_t)(plan.chunks + 1) * e_local * 4;
 }
 
 int b200moe_sort_tokens(const void* topk_ids, int ids_bits, int64_t ids_row_stride, int64_t tokens, int top_k, int e_local,
@@ -690,7 +730,7 @@ int b200moe_sort_tokens(const void* topk_ids, int ids_bits, int64_t ids_row_stri
   const SortPlan plan = sort_plan(tokens * top_k, rows);
   if (!plan.one_launch) {
     if (!workspace) return B200MOE_ERR_INVALID_ARGUMENT;
-    if (workspace_bytes < (size_t)plan.chunks * e_local * 4) return B200MOE_ERR_WORKSPACE_TOO_SMALL;
+    if (workspace_bytes < (size_t)(plan.chunks + 1) * e_local * 4) return B200MOE_ERR_WORKSPACE_TOO_SMALL;
   }
   int num_sms = 0;
   if ((rc = ensure_device(&num_sms)) != B200MOE_OK) return rc;
@@ -711,9 +751,10 @@ int b200moe_sort_tokens(const void* topk_ids, int ids_bits, int64_t ids_row_stri
   p.pos = pos;
   p.pair = pair;
   p.chunks = plan.chunks;
+  p.scanned = !plan.one_launch && (long long)plan.chunks * e_local > kSortScanCounters;
   p.chunk_counts = plan.one_launch ? nullptr : reinterpret_cast<int*>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  CUDA_TRY(plan.rounds == kSortRounds ? launch_sort<kSortRounds>(p, plan, st) : launch_sort<kSortManyRounds>(p, plan, st));
+  CUDA_TRY(launch_sort(p, plan, st));
   return B200MOE_OK;
 }
 

@@ -50,7 +50,7 @@ def check_order(order, ids, e_local, off, align):
     (1, 1, 1, 1, 0, 1), (1, 8, 256, 256, 0, 128), (5, 2, 4, 4, 0, 16), (16, 8, 256, 32, 64, 1), (33, 6, 160, 160, 0, 1),
     (100, 32, 64, 64, 0, 7), (129, 8, 256, 1, 255, 128), (400, 3, 1024, 1024, 0, 1), (1000, 8, 300, 257, 20, 128),
     (1023, 8, 256, 256, 0, 128), (1025, 8, 256, 256, 0, 1), (5000, 4, 700, 700, 0, 4), (9001, 8, 64, 64, 0, 1),
-    (70000, 8, 256, 256, 0, 128), (200001, 1, 1000, 900, 50, 1)])
+    (12000, 5, 1024, 1024, 0, 16), (100000, 7, 40, 33, 5, 1), (70000, 8, 256, 256, 0, 128), (200001, 1, 1000, 900, 50, 1)])
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 def test_sort(T, K, experts, e_local, off, align, dtype):
     ids = random_ids(T, K, experts, T + K, dtype)

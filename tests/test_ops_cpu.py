@@ -84,8 +84,8 @@ def test_sort_refusals(mem):
     assert lib.b200moe_sort_workspace_bytes(4, 8, 0) == INVALID and lib.b200moe_sort_workspace_bytes(4, 33, 8) == INVALID
     # none up to the pairs that one launch sorts (the host allocates none either), then a histogram for each chunk
     assert lib.b200moe_sort_workspace_bytes(2048, 8, 256) == 0 and F.ops._SORT_ONE_LAUNCH == 2048 * 8
-    assert lib.b200moe_sort_workspace_bytes(2049, 8, 256) == 9 * 256 * 4
-    assert lib.b200moe_sort_workspace_bytes(65537, 8, 10) == -(-65537 * 8 // 8192) * 10 * 4
+    assert lib.b200moe_sort_workspace_bytes(2049, 8, 256) == 10 * 256 * 4
+    assert lib.b200moe_sort_workspace_bytes(65537, 8, 10) == (-(-65537 * 8 // 2048) + 1) * 10 * 4
     assert call(_3=3000, _12=24000) == INVALID and call(_3=3000, _12=24000, _13=p, _14=12 * 16 * 4 - 1) == SPACE
 
 
