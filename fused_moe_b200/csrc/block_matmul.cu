@@ -816,7 +816,6 @@ extern "C" int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride, cons
   p.status = status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 
-
   p.split = 1;
   long long cost = mid_cost(m_tiles * n_tiles, p.kblocks, M < kTile ? M : kTile, 1, num_sms);
   for (int S : {2, 3, 4, 8}) {

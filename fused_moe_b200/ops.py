@@ -186,7 +186,7 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     dev = a.device
     if a_scale.device != dev or b.device != dev or b_scale.device != dev:
         raise _other_device(dev, a_scale=a_scale, b=b, b_scale=b_scale)
-    if (a_scale.requires_grad or b_scale.requires_grad) and torch.is_grad_enabled():
+    if (a_scale.requires_grad or b_scale.requires_grad or a.requires_grad or b.requires_grad) and torch.is_grad_enabled():
         raise _no_gradient("block_matmul")
     if a.dtype not in _CODES or b.dtype not in _CODES:
         raise TypeError(f"a and b must be float8_e4m3fn (or its uint8 bit pattern), got {a.dtype} and {b.dtype}")
@@ -224,7 +224,7 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
         return out
     st = _status.get(dev.index)
     if st is None and not torch.cuda.is_current_stream_capturing():   # (pinned memory cannot be had during a capture)
-        st = _status[dev.index] = _Status()
+        st = _status.setdefault(dev.index, _Status())
     if st is not None:
         st.raise_if_failed()
     _call("b200moe_block_matmul", dev.index, a_ptr, a_pitch, a_scale.data_ptr(), as_m, as_kb, b_ptr, b_pitch, b_scale.data_ptr(),
@@ -379,8 +379,8 @@ def permute(x: torch.Tensor, order: TokenOrder, *, out: Optional[torch.Tensor] =
     """Rows of x [T, H] in the sorted order, [order.rows, H]: ``y[pos[t, k]] = x[t]``, zeros in padding rows.
 
     Any type of 1, 2 or 4 bytes an element (e4m3 codes and their "tk" scales among them).  Rows behind the last expert are
-    zero too, except in an ``out`` of the caller's, where they stay as they were.  Differentiable for fp32, bf16 and fp16 x
-    (without ``out``): ``dx[t]`` is the sum of dy over the token's rows, in fp32, rounded once.
+    zero too, except in an ``out`` of the caller's (which must not overlap x), where they stay as they were.  Differentiable for
+    fp32, bf16 and fp16 x (without ``out``): ``dx[t]`` is the sum of dy over the token's rows, in fp32, rounded once.
     """
     if not x.is_cuda:
         raise _not_cuda(x, "x")
@@ -407,8 +407,8 @@ def unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tensor
     """Sums of each token's rows: ``out[t] = sum_k weights[t, k] * y[pos[t, k]]``, k ascending, fp32, rounded once to y's type.
 
     y [order.rows, H] fp32, bf16 or fp16; weights fp32 [T, top_k], or None for ones.  Choices that are not local add nothing (a
-    token without any is zero) whatever their weight.  Differentiable in y and weights (without ``out``): rows of dy that no
-    pair takes are zero, dw is 0 where the expert is not local.
+    token without any is zero) whatever their weight.  ``out`` must not overlap y.  Differentiable in y and weights (without
+    ``out``): rows of dy that no pair takes are zero, dw is 0 where the expert is not local.
     """
     if not y.is_cuda:
         raise _not_cuda(y, "y")

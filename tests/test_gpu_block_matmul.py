@@ -135,4 +135,6 @@ def test_empty_extents_and_refusals():
         F.block_matmul(a, sa, b, sb.cpu(), **ok)
     with pytest.raises(RuntimeError, match="no gradient"):
         F.block_matmul(a, sa.clone().requires_grad_(True), b, sb, **ok)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        F.block_matmul(a, sa, b.clone().view(torch.float8_e4m3fn).requires_grad_(True), sb, **ok)
     assert issubclass(MoEError, RuntimeError)
