@@ -336,14 +336,19 @@ def _unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tenso
     return res
 
 
+def _first_order(backward):
+    """``once_differentiable`` where a graph of the gradient is asked for; elsewhere without what that wrapper takes (4 us)."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+    return staticmethod(lambda ctx, grad: guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad))
+
+
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order):
         ctx.order = order
         return _permute(x, order, None)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dy):
         return _unpermute(dy, ctx.order, None, None), None
 
@@ -356,8 +361,7 @@ class _Unpermute(torch.autograd.Function):
         ctx.y_like = (y.shape, y.dtype)
         return _unpermute(y, order, weights, None)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dout):
         order, (y, weights) = ctx.order, ctx.saved_tensors
         (rows, H), dtype = ctx.y_like

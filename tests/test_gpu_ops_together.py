@@ -187,3 +187,16 @@ def test_offsets_beyond_32_bits():
     for got in (small[0], wide[-1, :128]):
         assert ((got.double() - ref).abs() <= 2.0 ** -13 * (one.double().abs() * so.double().t().repeat_interleave(128, 1))[:, ::512].sum()).all()
     assert not wide[:-1, :128].any()
+
+
+def test_second_derivatives_are_refused():
+    ids = torch.randint(0, 8, (64, 4), dtype=torch.int32, device=DEV)
+    order = F.sort_tokens(ids)
+    x = torch.randn(64, 32, device=DEV).requires_grad_(True)
+    y = torch.randn(order.rows, 32, device=DEV).requires_grad_(True)
+    w = torch.rand(64, 4, device=DEV).requires_grad_(True)
+    for out, leaf in ((F.permute(x, order), x), (F.unpermute(y, order, w), y)):
+        d = torch.ones_like(out).requires_grad_(True)
+        grad, = torch.autograd.grad(out, leaf, d, create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            grad.sum().backward()
