@@ -46,9 +46,6 @@ struct MatmulParams {
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, float a, float b, float c, float d) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, float a, float b, float c, float d) {
-  asm volatile("st.shared::cta.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
-}
 __device__ __forceinline__ float4 ld_shared_v4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cta.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -95,24 +92,117 @@ __device__ __forceinline__ void store4(const MatmulParams& p, int m, int n, floa
   }
 }
 
-// All 128 columns of a row from one thread, 32 bytes (a sector) at a time; rows of `out` start on such boundaries.
+// A row's word i (of 64 or 128), zero behind the last.
+template <bool F32>
+__device__ __forceinline__ uint32_t row_word(int out_dtype, const float2* v, int i) {
+  if (i >= (F32 ? kTile : kTile / 2)) return 0u;
+  return F32 ? __float_as_uint(i & 1 ? v[i / 2].y : v[i / 2].x) : pack16(out_dtype, v[i].x, v[i].y);
+}
+
+// `bytes` of a row from one thread, 32 bytes (a sector) at a time: up to the first such boundary, and behind the last, in parts
+// of 2, 4, 8 and 16 bytes, each where the address asks for it and the row has as many left.  What goes to a sector is taken out of
+// the words by a shift of up to seven of them (and, for 16-bit elements, half of one).  M x 2047 in bf16 (through shared memory by
+// single elements / so): M 8192, K 512 66 / 25 us, M 4096, K 2048 38 / 23; in fp32 49 / 30, 37 / 26.
+template <bool F32>
+__device__ __forceinline__ void store_row_shifted(uint8_t* dst, int out_dtype, const float2* v, int bytes) {
+  uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>(dst);
+  const bool c2 = !F32 && (at & 2) && bytes >= 2;
+  at += c2 ? 2 : 0, bytes -= c2 ? 2 : 0;
+  const bool c4 = (at & 4) && bytes >= 4;
+  at += c4 ? 4 : 0, bytes -= c4 ? 4 : 0;
+  const bool c8 = (at & 8) && bytes >= 8;
+  at += c8 ? 8 : 0, bytes -= c8 ? 8 : 0;
+  const bool c16 = (at & 16) && bytes >= 16;
+  bytes -= c16 ? 16 : 0;
+  uint32_t next[8];                                // the window's second half
+#pragma unroll
+  for (int j = 0; j < 8; ++j) next[j] = row_word<F32>(out_dtype, v, j);
+#pragma unroll
+  for (int i = -8; i < (F32 ? kTile : kTile / 2); i += 8) {
+    uint32_t x[16];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = next[j];
+      next[j] = row_word<F32>(out_dtype, v, i + 8 + j);
+      x[8 + j] = next[j];
+    }
+    if (i < 0) {                                   // before the first boundary
+      if (c2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)x[0];
+    }
+    if (!F32) {
+#pragma unroll
+      for (int j = 0; j < 15; ++j) x[j] = __funnelshift_r(x[j], x[j + 1], c2 ? 16 : 0);
+    }
+    if (i < 0) {
+      dst += c2 ? 2 : 0;
+      if (c4) *reinterpret_cast<uint32_t*>(dst) = x[0];
+      dst += c4 ? 4 : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 14; ++j) x[j] = c4 ? x[j + 1] : x[j];
+    if (i < 0) {
+      if (c8) *reinterpret_cast<uint2*>(dst) = make_uint2(x[0], x[1]);
+      dst += c8 ? 8 : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 12; ++j) x[j] = c8 ? x[j + 2] : x[j];
+    if (i < 0) {
+      if (c16) *reinterpret_cast<uint4*>(dst) = make_uint4(x[0], x[1], x[2], x[3]);
+      dst += c16 ? 16 : 0;
+      continue;                                    // (the window stood still: its second half is the row's first eight words)
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = c16 ? x[j + 4] : x[j];
+    if (bytes >= 32) {
+      const uint32_t w[8] = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+      st_global_v8(dst, w);
+    } else if (bytes > 0) {
+      uint8_t* d = dst;
+      if (bytes & 16) {
+        *reinterpret_cast<uint4*>(d) = make_uint4(x[0], x[1], x[2], x[3]);
+        x[0] = x[4], x[1] = x[5], x[2] = x[6], x[3] = x[7];
+        d += 16;
+      }
+      if (bytes & 8) {
+        *reinterpret_cast<uint2*>(d) = make_uint2(x[0], x[1]);
+        x[0] = x[2], x[1] = x[3];
+        d += 8;
+      }
+      if (bytes & 4) {
+        *reinterpret_cast<uint32_t*>(d) = x[0];
+        x[0] = x[1];
+        d += 4;
+      }
+      if (bytes & 2) *reinterpret_cast<uint16_t*>(d) = (uint16_t)x[0];
+    }
+    dst += 32;
+    bytes -= 32;
+  }
+}
+
+// Columns [n, n + 128) of row m, of which those below N exist, from one thread.
 __device__ __forceinline__ void store_row128(const MatmulParams& p, int m, int n, const float2* v) {
-  if (p.out_dtype == B200MOE_F32) {
-    float* dst = reinterpret_cast<float*>(p.out) + (size_t)m * p.out_stride + n;
+  const int cols = min(kTile, p.N - n);
+  if (m >= p.M || cols <= 0) return;
+  const bool f32 = p.out_dtype == B200MOE_F32;
+  uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + ((size_t)m * p.out_stride + n) * (f32 ? 4 : 2);
+  if (p.vec_out < 2 || cols < kTile) {
+    if (f32) store_row_shifted<true>(dst, p.out_dtype, v, 4 * cols);
+    else store_row_shifted<false>(dst, p.out_dtype, v, 2 * cols);
+  } else if (f32) {
 #pragma unroll
     for (int i = 0; i < 64; i += 4) {
       uint32_t w[8];
       memcpy(w, v + i, 32);
-      st_global_v8(dst + 2 * i, w);
+      st_global_v8(dst + 8 * i, w);
     }
   } else {
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (size_t)m * p.out_stride + n;
 #pragma unroll
     for (int i = 0; i < 64; i += 8) {
       uint32_t w[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = pack16(p.out_dtype, v[i + j].x, v[i + j].y);
-      st_global_v8(dst + 2 * i, w);
+      st_global_v8(dst + 4 * i, w);
     }
   }
 }
@@ -264,31 +354,26 @@ constexpr int kMidLaunchRegs = 128, kMidCtrlRegs = 48, kMidPromoRegs = 208;
 static_assert(128 * (kMidLaunchRegs - kMidCtrlRegs) >= 128 * (kMidPromoRegs - kMidLaunchRegs),
               "setmaxnreg.inc would wait for registers that nobody releases");
 
-// The sum of a split product, and the way of a tile into rows that are not aligned.  A row's 32 vectors of four columns are divided
-// over the cluster's CTAs: each receives its part of every CTA's partial sums in its ring (idle by then), adds them in the order
-// of the ranks and stores them, neighbouring lanes neighbouring rows' vectors.
+// The sum of a split product.  A row's 32 vectors of four columns are divided over the cluster's CTAs: each receives its part of
+// every CTA's partial sums in its ring (idle by then), adds them in the order of the ranks and stores them, neighbouring lanes
+// neighbouring rows' vectors.
 template <int S>
 __device__ __forceinline__ void join_split(const MatmulParams& p, const float2* acc, uint32_t smem_base, int thread, int rows, int m0,
                                            int n0) {
   constexpr int kMost = (kTile / 4 + S - 1) / S;   // vectors of a part
-  const int me = S > 1 ? (int)cluster_rank() : 0;
+  const int me = (int)cluster_rank();
   if (thread < rows) {
 #pragma unroll
     for (int c = 0; c < kTile / 4; ++c) {
       const int j = ((c + 1) * S - 1) / (kTile / 4);   // the CTA whose part [32 j / S, 32 (j + 1) / S) has c
       const uint32_t at = smem_base + ((me * kMost + c - kTile / 4 * j / S) * kTile + thread) * 16;
       const float2 x = acc[2 * c], y = acc[2 * c + 1];
-      if (S > 1) st_cluster_v4(map_to_rank(at, (uint32_t)j), x.x, x.y, y.x, y.y);
-      else st_shared_v4(at, x.x, x.y, y.x, y.y);
+      st_cluster_v4(map_to_rank(at, (uint32_t)j), x.x, x.y, y.x, y.y);
     }
   }
   __syncwarp();
-  if (S > 1) {
-    cluster_arrive();
-    cluster_wait();
-  } else {
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-  }
+  cluster_arrive();
+  cluster_wait();
   // a quarter-warp reads eight rows of one vector column (no bank twice); four vector columns of a row are stored together
   const int first = kTile / 4 * me / S, n = kTile / 4 * (me + 1) / S - first;
   const int row8 = thread & 7, c4 = (thread >> 3) & 3, warp = thread >> 5, groups = (rows + 7) / 8;
@@ -447,12 +532,7 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
     }
     const int thread = threadIdx.x - 128;
     if (split == 1) {
-      if (p.vec_out == 2 && n0 + kTile <= p.N) {
-        if (row < p.M) store_row128(p, row, n0, acc);
-      } else {
-        // through the ring: the last MMAs have read it (their accumulators were waited for)
-        join_split<1>(p, acc, smem_base, thread, rows, m0, n0);
-      }
+      store_row128(p, row, n0, acc);
     } else {
       // every CTA's ring is idle behind this barrier; the promotion warps then exchange the partial sums
       __syncwarp();
@@ -484,9 +564,7 @@ constexpr int kPairThreads = 384;                // warps 0: TMA, 1-2: MMA issue
 constexpr int kPairStages = 5;
 static_assert(kPairStages >= 5, "what an issuer knows of a stage's use before (see there)");
 constexpr int kPairStageBytes = kStageBytes;     // a CTA's part: 128 rows of A, 2 x 64 rows of B
-constexpr int kStagePitch = 33;                  // floats of a row of a warp's staging square (odd: no bank twice)
-constexpr int kPairStagingBytes = 8 * 32 * kStagePitch * 4;
-constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + kPairStagingBytes + kScaleRing * 2 * kTile * 4 + 1024;
+constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + kScaleRing * 2 * kTile * 4 + 1024;
 constexpr int kPairLaunchRegs = 168, kPairCtrlRegs = 72, kPairPromoRegs = 216;
 static_assert(128 * (kPairLaunchRegs - kPairCtrlRegs) >= 256 * (kPairPromoRegs - kPairLaunchRegs),
               "setmaxnreg.inc would wait for registers that nobody releases");
@@ -595,7 +673,7 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
   cluster_wait();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const uint32_t factors = smem_base + S * kPairStageBytes + kPairStagingBytes;   // [kScaleRing][2][128]
+  const uint32_t factors = smem_base + S * kPairStageBytes;   // [kScaleRing][2][128]
   const int tiles = p.m_tiles * p.n_tiles, first = blockIdx.x >> 1, stride = gridDim.x >> 1, kblocks = p.kblocks;
   chain_wait();
   chain_release();
@@ -676,7 +754,6 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
     const int pw = warp - 4, half = pw >> 2, q = pw & 3;
     const uint32_t read = map_to_rank(count_read + 8 * half, 0), slot = map_to_rank(bar_slot, rank);
     const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + half * 2 * kTile;
-    const uint32_t staging = smem_base + S * kPairStageBytes + pw * (32 * kStagePitch * 4);
     uint32_t it = 0, seen_f = 0, seen_d = 0;   // seen: the coming K block's factors, accumulator are known to be there (looked at below)
     bool alive = true;
     for (int tile = first; tile < tiles && alive; tile += stride) {
@@ -709,31 +786,7 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
         seen_d = __all_sync(0xffffffffu, seen_d);
       }
       if (!alive) break;
-      if (p.vec_out == 2 && n0 + kTile <= p.N) {
-        if (m0 + lane < p.M) store_row128(p, m0 + lane, n0, acc);
-      } else {
-        // 32 x 32 squares through shared memory, so that a warp stores a row's neighbours
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            asm volatile("st.shared::cta.f32 [%0], %1;" ::"r"(staging + (lane * kStagePitch + 2 * j) * 4), "f"(acc[16 * c + j].x) : "memory");
-            asm volatile("st.shared::cta.f32 [%0], %1;" ::"r"(staging + (lane * kStagePitch + 2 * j + 1) * 4), "f"(acc[16 * c + j].y) : "memory");
-          }
-          __syncwarp();
-          const int n = n0 + c * 32 + lane;
-          for (int r = 0; r < 32; ++r) {
-            float v;
-            asm volatile("ld.shared::cta.f32 %0, [%1];" : "=f"(v) : "r"(staging + (r * kStagePitch + lane) * 4) : "memory");
-            if (n < p.N && m0 + r < p.M) {
-              const size_t at = (size_t)(m0 + r) * p.out_stride + n;
-              if (p.out_dtype == B200MOE_F32) reinterpret_cast<float*>(p.out)[at] = v;
-              else reinterpret_cast<uint16_t*>(p.out)[at] = (uint16_t)pack16(p.out_dtype, v, 0.f);
-            }
-          }
-          __syncwarp();
-        }
-      }
+      store_row128(p, m0 + lane, n0, acc);
     }
   }
   tc_fence_before();

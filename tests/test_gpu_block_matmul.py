@@ -89,6 +89,21 @@ def test_strides_of_everything():
         assert torch.equal(host[:, 1:1 + N], ref.to(dt)) and (host[:, 0] == 7).all() and (host[:, 1 + N:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(300, 77, 128), (130, 256, 64), (70, 200, 2048), (3000, 1, 128), (4200, 1301, 256), (2600, 2176, 400)])
+def test_result_rows_that_start_anywhere(M, N, K, dtype):
+    """Rows of the result on every boundary of their elements, by start and by pitch; what lies beside them stays."""
+    a, sa, b, sb = small_whole_numbers(M, N, K, 2)
+    ea, eb = expand(sa, sb, N, K)
+    ref = ((a.double() * ea) @ (b.double() * eb).t()).to(dtype)
+    for start, pitch in [(s, N + 17 + s % 2) for s in range(17)] + [(s, -(-(N + 16) // 32) * 32) for s in (0, 1, 4, 8, 15, 16)]:
+        host = torch.full((M + 2, pitch), 7.0, device=DEV, dtype=dtype)
+        F.block_matmul(a, sa, b, sb, scale_layout="tk", out=host[1:-1, start:start + N])
+        assert torch.equal(host[1:-1, start:start + N], ref), (start, pitch)
+        host[1:-1, start:start + N] = 7.0
+        assert (host == 7).all(), (start, pitch)
+
+
 @pytest.mark.parametrize("M", [3, 40, 200, 700])
 def test_not_a_number_stays_in_its_row_and_column(M):
     N, K = 300, 1024
