@@ -105,12 +105,12 @@ sort_scan_kernel(const __grid_constant__ SortParams p) {
     before += w < warp ? n : 0;
     total += n;
   }
-  for (int c = c0; c < c1; c += 16) {
-    int n[16];
+  for (int c = c0; c < c1; c += 8) {
+    int n[8];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) n[j] = c + j < c1 ? p.chunk_counts[(size_t)(c + j) * E + x] : 0;
+    for (int j = 0; j < 8; ++j) n[j] = c + j < c1 ? p.chunk_counts[(size_t)(c + j) * E + x] : 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 8; ++j) {
       if (c + j < c1) p.chunk_counts[(size_t)(c + j) * E + x] = before;
       before += n[j];
     }
@@ -423,12 +423,12 @@ __device__ __forceinline__ void store_pack(P* p, const P& v) {
 
 constexpr int kSumBatch = 8;                     // rows of a token in flight together
 
-// A CTA takes a token's output row, or one of `segments` parts of it: the rows' addresses are then known for the whole row, and eight
-// loads a thread are in flight.  (A warp for each 512 bytes of an output row, which has to fetch the positions first, reached 3.5
-// TB/s of 14 KB rows, this 6.)  AHEAD: four CTAs an SM take one row after another, with the next one's positions on their way
-// meanwhile.  us, without / with: 8192 rows of 2048 bf16 62 / 53, 16384 of 512 69 / 49, 4096 of 7168 89 / 86; 4097 of 2048 fp32 47 /
+// A GROUP of threads takes a token's output row, or one of `segments` parts of it: the rows' addresses are then known for the whole
+// row, and eight loads a thread are in flight (U times as many where a load brings less than 16 bytes).  (A warp for each 512 bytes
+// of an output row, which has to fetch the positions first, reached 3.5 TB/s of 14 KB rows, this 6.)  AHEAD: four CTAs an SM take
+// one row after another, with the next one's positions on their way meanwhile.  us, without / with: 8192 rows of 2048 bf16 62 / 53, 16384 of 512 69 / 49, 4096 of 7168 89 / 86; 4097 of 2048 fp32 47 /
 // 57, of 7168 153 / 184: fp32, whose sums take fewer registers, has six CTAs on an SM without it (with four of them 58 us).
-template <typename T, int N, int U, bool AHEAD>
+template <typename T, int N, int U, int GROUP, bool AHEAD>
 __global__ void __launch_bounds__(kMoveThreads, AHEAD ? 4 : 6)
 unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restrict__ pos, const float* __restrict__ weights,
                  long long w_stride, T* __restrict__ out, long long out_stride, int items, int top_k, int row_vecs,
@@ -446,7 +446,9 @@ unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restr
       w[j] = weights && k0 + j < top_k ? __ldg(weights + (size_t)t * w_stride + k0 + j) : 1.f;
     }
   };
-  int item = blockIdx.x;                         // (below `items`)
+  const int lane = threadIdx.x % GROUP;
+  int item = blockIdx.x * (kMoveThreads / GROUP) + threadIdx.x / GROUP;
+  if (item >= items) return;
   fetch(item / segments, 0);
   do {
     const int t = item / segments, v_begin = (item - t * segments) * segment_vecs, v_end = min(v_begin + segment_vecs, row_vecs);
@@ -461,22 +463,24 @@ unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restr
       }
     };
     use();
-    item += gridDim.x;
+    item += gridDim.x * (kMoveThreads / GROUP);
     if (AHEAD && top_k <= kSumBatch && item < items) fetch(item / segments, 0);
-    for (int v = v_begin + threadIdx.x; v < v_end; v += U * kMoveThreads) {
+    for (int v = v_begin + lane; v < v_end; v += U * GROUP) {
       float acc[U][N];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
+      int at[U];                                   // (loads behind the end repeat the last: one that only some threads make waits alone)
+#pragma unroll
+      for (int u = 0; u < U; ++u) at[u] = U == 1 ? v : min(v + u * GROUP, v_end - 1);
       for (int k0 = 0;;) {
         P x[kSumBatch][U];
 #pragma unroll
         for (int j = 0; j < kSumBatch; ++j)
           if (src[j]) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-              if (U == 1 || v + u * kMoveThreads < v_end) x[j][u] = load_pack(src[j] + v + u * kMoveThreads);
+            for (int u = 0; u < U; ++u) x[j][u] = load_pack(src[j] + at[u]);
           }
 #pragma unroll
         for (int j = 0; j < kSumBatch; ++j)
@@ -497,7 +501,7 @@ unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restr
         P r;
 #pragma unroll
         for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(acc[u][i]);
-        if (U == 1 || v + u * kMoveThreads < v_end) store_pack(dst + v + u * kMoveThreads, r);
+        if (U == 1 || v + u * GROUP < v_end) store_pack(dst + v + u * GROUP, r);
       }
     }
     if (AHEAD && top_k > kSumBatch && item < items) fetch(item / segments, 0);
@@ -524,8 +528,8 @@ struct UnpermuteGrad {
 
 // One CTA per token: its row of dout is read once (top_k <= 8), each sorted row of y read and of dy written once; the dots are
 // summed by shuffles and over the four warps in a fixed order.
-template <typename T, int N>
-__global__ void __launch_bounds__(kMoveThreads, 5)
+template <typename T, int N, int U>
+__global__ void __launch_bounds__(kMoveThreads, U > 1 ? 4 : 5)
 unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long items) {
   using P = Pack<T, N>;
   constexpr int kWarps = kMoveThreads / 32;
@@ -550,26 +554,40 @@ unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long item
         wt[j] = there && p.weights ? p.weights[t * p.w_stride + k0 + j] : 1.f;
         dot[j] = 0.f;
       }
-      for (int v = threadIdx.x; v < p.row_vecs; v += kMoveThreads) {
-        const P d = load_pack(dout + v);
-        P x[kSumBatch];
+      for (int v = threadIdx.x; v < p.row_vecs; v += U * kMoveThreads) {
+        // (loads behind the end repeat the last vector; neither stored nor summed)
+        int at[U];
+        bool there[U];
+        P d[U], x[kSumBatch][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          at[u] = U == 1 ? v : min(v + u * kMoveThreads, p.row_vecs - 1);
+          there[u] = U == 1 || v + u * kMoveThreads < p.row_vecs;
+          d[u] = load_pack(dout + at[u]);
+        }
         if (p.dw) {
 #pragma unroll
           for (int j = 0; j < kSumBatch; ++j)
-            if (row[j] >= 0) x[j] = load_pack(reinterpret_cast<const P*>(p.y + row[j] * p.y_stride) + v);
+            if (row[j] >= 0) {
+#pragma unroll
+              for (int u = 0; u < U; ++u) x[j][u] = load_pack(reinterpret_cast<const P*>(p.y + row[j] * p.y_stride) + at[u]);
+            }
         }
 #pragma unroll
         for (int j = 0; j < kSumBatch; ++j) {
           if (row[j] < 0) continue;
-          if (p.dw) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) dot[j] = fmaf(to_float(d.v[i]), to_float(x[j].v[i]), dot[j]);
-          }
-          if (p.dy) {
-            P r;
+          for (int u = 0; u < U; ++u) {
+            if (p.dw && there[u]) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(wt[j] * to_float(d.v[i]));
-            store_pack(reinterpret_cast<P*>(p.dy + row[j] * p.dy_stride) + v, r);
+              for (int i = 0; i < N; ++i) dot[j] = fmaf(to_float(d[u].v[i]), to_float(x[j][u].v[i]), dot[j]);
+            }
+            if (p.dy && there[u]) {
+              P r;
+#pragma unroll
+              for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(wt[j] * to_float(d[u].v[i]));
+              store_pack(reinterpret_cast<P*>(p.dy + row[j] * p.dy_stride) + at[u], r);
+            }
           }
         }
       }
@@ -604,23 +622,35 @@ cudaError_t launch_permute_rows(const RowMove& p, int num_sms, cudaStream_t stre
                         stream, p, segments, move_items, items);
 }
 
+template <typename T, int N, int U, int GROUP>
+cudaError_t launch_unpermute_group(const void* y, long long y_stride, const int* pos, const float* weights, long long w_stride, void* out,
+                                   long long out_stride, int tokens, int top_k, int row_vecs, int num_sms, cudaStream_t stream) {
+  constexpr bool kAhead = sizeof(T) == 2;
+  constexpr int kGroups = kMoveThreads / GROUP;
+  // one group a token, more where that leaves SMs without one
+  const int pieces = (row_vecs + GROUP - 1) / GROUP;
+  int segments = (int)(((kAhead ? 4ll : 8ll) * kGroups * num_sms + tokens - 1) / tokens);
+  if (segments > pieces) segments = pieces;
+  const int segment_vecs = (pieces + segments - 1) / segments * GROUP;
+  segments = (row_vecs + segment_vecs - 1) / segment_vecs;
+  const long long items = (long long)tokens * segments;
+  if (items > 0x7fffffffll - 32ll * num_sms) return cudaErrorInvalidValue;   // (a token in parts: few tokens)
+  return launch_chained(unpermute_kernel<T, N, U, GROUP, kAhead>, dim3(grid_for((items + kGroups - 1) / kGroups, kAhead ? 4ll * num_sms : items)),
+                        dim3(kMoveThreads), 0, stream, reinterpret_cast<const T*>(y), y_stride, pos, weights, w_stride,
+                        reinterpret_cast<T*>(out), out_stride, (int)items, top_k, row_vecs, segments, segment_vecs);
+}
+
 template <typename T, int N>
 cudaError_t launch_unpermute(const void* y, long long y_stride, const int* pos, const float* weights, long long w_stride, void* out,
                              long long out_stride, int tokens, int top_k, int hidden, int num_sms, cudaStream_t stream) {
-  constexpr int U = sizeof(T) * N == 16 ? 1 : sizeof(T) * N == 4 ? 2 : 4;   // loads of fewer bytes: more of them in flight
+  // loads of fewer bytes: more of them in flight (as many as leave the registers without spills)
+  constexpr int U = sizeof(T) * N == 16 ? 1 : sizeof(T) == 4 ? 2 : N == 2 ? 3 : 4;
   const int row_vecs = hidden / N;
-  // one CTA a token, more where that leaves SMs without one
-  const int pieces = (row_vecs + kMoveThreads - 1) / kMoveThreads;
-  constexpr bool kAhead = sizeof(T) == 2;
-  int segments = (int)(((kAhead ? 4ll : 8ll) * num_sms + tokens - 1) / tokens);
-  if (segments > pieces) segments = pieces;
-  const int segment_vecs = (pieces + segments - 1) / segments * kMoveThreads;
-  segments = (row_vecs + segment_vecs - 1) / segment_vecs;
-  const long long items = (long long)tokens * segments;
-  if (items > 0x7fffffffll - 8ll * num_sms) return cudaErrorInvalidValue;   // (a token in parts: few tokens)
-  return launch_chained(unpermute_kernel<T, N, U, kAhead>, dim3(grid_for(items, kAhead ? 4ll * num_sms : items)), dim3(kMoveThreads), 0, stream,
-                        reinterpret_cast<const T*>(y), y_stride, pos, weights, w_stride, reinterpret_cast<T*>(out), out_stride,
-                        (int)items, top_k, row_vecs, segments, segment_vecs);
+  // Short rows leave threads of a group of 128 idle.  us, groups of 32 / of 128: bf16 16384 rows of 512 27 / 47, 8192 of 1536 41 / 47, of
+  // 2048 54 / 52, 4096 of 602 11 / 14, of 7168 91 / 86; fp32 16384 rows of 512, two choices 22 / 31, 8192 of 1024 52 / 46.
+  const bool small = sizeof(T) == 2 ? row_vecs < 2 * U * kMoveThreads : row_vecs <= U * kMoveThreads;
+  auto go = small ? launch_unpermute_group<T, N, U, 32> : launch_unpermute_group<T, N, U, kMoveThreads>;
+  return go(y, y_stride, pos, weights, w_stride, out, out_stride, tokens, top_k, row_vecs, num_sms, stream);
 }
 
 // elements of a vector: 16 bytes, 4 bytes or one element, as far as all rows start on such a boundary (`bits`: addresses
@@ -646,7 +676,10 @@ cudaError_t launch_unpermute_grad(UnpermuteGrad<T> p, int hidden, int num_sms, c
   constexpr int kWarps = kMoveThreads / 32;
   const long long items = p.tokens + (p.dy ? (p.rows + kZeroRows * kWarps - 1) / (kZeroRows * kWarps) : 0);
   if (items == 0) return cudaSuccess;
-  return launch_chained(unpermute_grad_kernel<T, N>, dim3(grid_for(items, 64ll * num_sms)), dim3(kMoveThreads), 0, stream, p, items);
+  // single elements: more loads in flight.  us, one at a time / four: 2048 tokens x 8 of 4097 bf16 104 / 80, fp32 132 / 108; pairs of
+  // 16-bit elements gain nothing
+  constexpr int U = N == 1 ? 4 : 1;
+  return launch_chained(unpermute_grad_kernel<T, N, U>, dim3(grid_for(items, 64ll * num_sms)), dim3(kMoveThreads), 0, stream, p, items);
 }
 
 template <typename T>
