@@ -6,8 +6,8 @@
 //
 // Bound by HBM: every input byte is read once, one byte per element and four per block are written.  Sixteen lanes
 // take a block, eight elements each (16 bytes of a 16-bit type), so that a lane's part stays in registers between the maximum
-// and the division.  A CTA takes eight blocks of eight rows: every half-warp has four of them in flight, reads come in pieces of
-// 2 KB, and scales leave by the sector in either layout.
+// and the division.  A CTA takes eight blocks of eight rows (fewer blocks of more rows, see quantize_log_width): every half-warp has
+// four of them in flight, reads come in pieces of 2 KB, and scales leave by the sector in either layout.
 #include "common.cuh"
 #include "host.cuh"
 #include "kernels.cuh"
@@ -18,11 +18,9 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantHalves = kQuantThreads / 16;   // half-warps of a CTA
-constexpr int kQuantBlocks = 8;                    // blocks of a CTA's tile in each of its rows
 // Blocks of a half-warp, all in flight: four, two behind a SwiGLU, whose exponentials take as long as memory does (with twice
-// as many CTAs one computes while another loads: 14.4 us instead of 14.7 for 4099 x 2048), and the rows of a CTA that go with them.
+// as many CTAs one computes while another loads: 14.4 us instead of 14.7 for 4099 x 2048).
 __host__ __device__ constexpr int quant_units(bool swiglu) { return swiglu ? 2 : 4; }
-__host__ __device__ constexpr int quant_rows(bool swiglu) { return quant_units(swiglu) * kQuantHalves / kQuantBlocks; }
 constexpr float kAmaxMin = 1e-12f;
 
 // A NaN stays one: it makes its block's scale, and so all codes of the block, NaN (an infinity makes the scale infinite),
@@ -60,6 +58,7 @@ template <> struct Elem<__half> {
     return r;
   }
   static __device__ float lower(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)v)); }
+  static __device__ float upper(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
 };
 template <> struct Elem<__nv_bfloat16> {
   static constexpr bool kShort = true;
@@ -70,6 +69,7 @@ template <> struct Elem<__nv_bfloat16> {
     return r;
   }
   static __device__ float lower(uint32_t v) { return __uint_as_float(v << 16); }
+  static __device__ float upper(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 };
 
 // A lane's eight elements of a block: neighbours, by 16-byte loads (VEC), or every sixteenth, so that a half-warp's lanes take
@@ -87,6 +87,16 @@ struct Raw8 {
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = 16 * i < left ? p[16 * i] : T(0.f);
+    }
+  }
+  // (16-bit elements out of whole words)
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (Elem<T>::kShort) {
+      uint32_t w;
+      memcpy(&w, v + (i & ~1), 4);
+      return i & 1 ? Elem<T>::upper(w) : Elem<T>::lower(w);
+    } else {
+      return Elem<T>::get(v[i]);
     }
   }
 };
@@ -108,20 +118,22 @@ __device__ __forceinline__ float2 div2_rn_any(float2 x, float d, float inv) {
 template <typename T, bool SWIGLU, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads)
 quantize_kernel(const T* __restrict__ x, long long x_stride, int rows, int cols, int kblocks, uint8_t* __restrict__ codes,
-                long long codes_stride, float* __restrict__ scale, long long s_stride_t, long long s_stride_kb) {
-  constexpr int kQuantUnits = quant_units(SWIGLU), kQuantRows = quant_rows(SWIGLU);
-  __shared__ float s_scale[kQuantRows * kQuantBlocks];
+                long long codes_stride, float* __restrict__ scale, long long s_stride_t, long long s_stride_kb, int log_width) {
+  constexpr int kQuantUnits = quant_units(SWIGLU), kTileBlocks = kQuantUnits * kQuantHalves;
+  const int width = 1 << log_width, step = kQuantHalves >> log_width, tile_rows = kTileBlocks >> log_width;   // (step: rows of a pass)
+  __shared__ float s_scale[kTileBlocks];
   chain_wait();
   chain_release();
-  const int groups = (kblocks + kQuantBlocks - 1) / kQuantBlocks;
-  const int kb0 = (int)(blockIdx.x % groups) * kQuantBlocks, row0 = (int)(blockIdx.x / groups) * kQuantRows;
+  const int groups = (kblocks + width - 1) >> log_width;
+  const int kb0 = (int)(blockIdx.x % groups) << log_width, row0 = (int)(blockIdx.x / groups) * tile_rows;
   const int part = threadIdx.x & 15, hw = threadIdx.x >> 4;
-  const int col = (kb0 + hw % kQuantBlocks) * kBlockK + (VEC ? part * 8 : part);
+  const int my_kb = hw & (width - 1), my_row = hw >> log_width;
+  const int col = (kb0 + my_kb) * kBlockK + (VEC ? part * 8 : part);
   const int left = cols - col;                     // columns from this lane's first on
   Raw8<T, VEC> a[kQuantUnits], b[SWIGLU ? kQuantUnits : 1];
 #pragma unroll
   for (int r = 0; r < kQuantUnits; ++r) {
-    const int row = row0 + r * (kQuantHalves / kQuantBlocks) + hw / kQuantBlocks;
+    const int row = row0 + r * step + my_row;
     const T* p = x + (size_t)row * x_stride + col;
     a[r].load(p, row < rows ? left : 0);
     if (SWIGLU) b[r].load(p + cols, row < rows ? left : 0);
@@ -154,9 +166,9 @@ quantize_kernel(const T* __restrict__ x, long long x_stride, int rows, int cols,
       m[r] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float x = Elem<T>::get(a[r].v[i]);
+        float x = a[r].get(i);
         if (SWIGLU) {
-          const float u = Elem<T>::get(b[r].v[i]);
+          const float u = b[r].get(i);
           // (a quarter of the divisor: its reciprocal is a normal number for all that expf gives below infinity)
           x *= 0.25f * u * rcp_from_quarter(fmaf(expf(-u), 0.25f, 0.25f));
         }
@@ -171,14 +183,14 @@ quantize_kernel(const T* __restrict__ x, long long x_stride, int rows, int cols,
   const float mine = kQuantUnits == 4 && (part & 2) ? (part & 1 ? m[kQuantUnits - 1] : m[kQuantUnits - 2]) : (part & 1 ? m[1] : m[0]);
   const float my_s = (mine < kAmaxMin ? kAmaxMin : mine) / 448.0f, my_inv = __frcp_rn(my_s);
   if (part < kQuantUnits)
-    s_scale[(hw % kQuantBlocks) * kQuantRows + part * (kQuantHalves / kQuantBlocks) + hw / kQuantBlocks] = my_s;
+    s_scale[my_kb * tile_rows + part * step + my_row] = my_s;
 #pragma unroll
   for (int r = 0; r < kQuantUnits; ++r) {
-    const int row = row0 + r * (kQuantHalves / kQuantBlocks) + hw / kQuantBlocks;
+    const int row = row0 + r * step + my_row;
     const float s = __shfl_sync(0xffffffffu, my_s, r, 16), inv = __shfl_sync(0xffffffffu, my_inv, r, 16);
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = kPacked ? Elem<T>::get(a[r].v[i]) : v[kPacked ? 0 : r][i];
+    for (int i = 0; i < 8; ++i) x[i] = kPacked ? a[r].get(i) : v[kPacked ? 0 : r][i];
     float2 q[4];
     if (s < INFINITY) {
 #pragma unroll
@@ -204,15 +216,22 @@ quantize_kernel(const T* __restrict__ x, long long x_stride, int rows, int cols,
   }
   __syncthreads();
   // neighbouring threads neighbouring rows of the [K/128, T] layout, neighbouring blocks of the other
-  if (threadIdx.x < kQuantRows * kQuantBlocks) {
-    const int i = threadIdx.x, rt = s_stride_t == 1 ? i % kQuantRows : i / kQuantBlocks, kb = s_stride_t == 1 ? i / kQuantRows : i % kQuantBlocks;
+  if (threadIdx.x < kTileBlocks) {
+    const int i = threadIdx.x;
+    const int rt = s_stride_t == 1 ? i & (tile_rows - 1) : i >> log_width, kb = s_stride_t == 1 ? i / tile_rows : i & (width - 1);
     if (row0 + rt < rows && kb0 + kb < kblocks)
-      scale[(size_t)(row0 + rt) * s_stride_t + (size_t)(kb0 + kb) * s_stride_kb] = s_scale[kb * kQuantRows + rt];
+      scale[(size_t)(row0 + rt) * s_stride_t + (size_t)(kb0 + kb) * s_stride_kb] = s_scale[kb * tile_rows + rt];
   }
 }
 
+// Blocks that a CTA's tile has of a row: the largest power of two up to eight that leaves no tile with blocks behind the row's end.
+// us, bf16, with 1, 2, 4, 8: 8192 x 7168 32.5, 32.2, 31.9, 31.7; 8192 x 4480 21.1, 21.5, 21.3, 23.0; 32768 x 1152 21.8, 23.3, 26.4, 33.0;
+// 65536 x 512 19.1, 18.9, 18.7, 32.2; 262144 x 128 18.7, 32.2, 59.1, 115.
+int quantize_log_width(int kblocks) { return kblocks % 8 == 0 ? 3 : kblocks % 4 == 0 ? 2 : kblocks % 2 == 0 ? 1 : 0; }
+
 long long quantize_grid(int rows, int kblocks, bool swiglu) {
-  return (long long)((kblocks + kQuantBlocks - 1) / kQuantBlocks) * (((long long)rows + quant_rows(swiglu) - 1) / quant_rows(swiglu));
+  const int log_width = quantize_log_width(kblocks), tile_rows = quant_units(swiglu) * kQuantHalves >> log_width;
+  return (long long)((kblocks + (1 << log_width) - 1) >> log_width) * (((long long)rows + tile_rows - 1) / tile_rows);
 }
 
 template <typename T, bool SWIGLU>
@@ -225,7 +244,7 @@ cudaError_t launch_one(const void* x, long long x_stride, int rows, int cols, ui
                    reinterpret_cast<uintptr_t>(codes) % 8 == 0 && codes_stride % 8 == 0;
   auto* kern = vec ? quantize_kernel<T, SWIGLU, true> : quantize_kernel<T, SWIGLU, false>;
   return launch_chained(kern, dim3((unsigned)grid), dim3(kQuantThreads), 0, stream, reinterpret_cast<const T*>(x), x_stride,
-                        rows, cols, kblocks, codes, codes_stride, scale, s_stride_t, s_stride_kb);
+                        rows, cols, kblocks, codes, codes_stride, scale, s_stride_t, s_stride_kb, quantize_log_width(kblocks));
 }
 
 template <typename T>

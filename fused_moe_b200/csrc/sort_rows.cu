@@ -391,9 +391,23 @@ permute_kernel(const __grid_constant__ RowMove p, int segments, long long move_i
 
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 
+template <typename T> struct is_bf16 { static constexpr bool value = false; };
+template <> struct is_bf16<__nv_bfloat16> { static constexpr bool value = true; };
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+// Element i of a pack; bf16 out of whole words, one instruction each.  (By single elements the gradient of 4096 tokens of 2048 takes
+// 54 us instead of 47, of 16384 of 512 71 instead of 53.)
+template <typename T, int N>
+__device__ __forceinline__ float elem(const Pack<T, N>& p, int i) {
+  if constexpr (N % 2 == 0 && sizeof(T) == 2 && is_bf16<T>::value) {
+    uint32_t w;
+    memcpy(&w, p.v + (i & ~1), 4);
+    return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+  } else {
+    return to_float(p.v[i]);
+  }
+}
 template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
@@ -426,8 +440,9 @@ constexpr int kSumBatch = 8;                     // rows of a token in flight to
 // A GROUP of threads takes a token's output row, or one of `segments` parts of it: the rows' addresses are then known for the whole
 // row, and eight loads a thread are in flight (U times as many where a load brings less than 16 bytes).  (A warp for each 512 bytes
 // of an output row, which has to fetch the positions first, reached 3.5 TB/s of 14 KB rows, this 6.)  AHEAD: four CTAs an SM take
-// one row after another, with the next one's positions on their way meanwhile.  us, without / with: 8192 rows of 2048 bf16 62 / 53, 16384 of 512 69 / 49, 4096 of 7168 89 / 86; 4097 of 2048 fp32 47 /
-// 57, of 7168 153 / 184: fp32, whose sums take fewer registers, has six CTAs on an SM without it (with four of them 58 us).
+// one row after another, with the next one's positions on their way meanwhile.  us, without / with: 8192 rows of 2048 bf16 62 /
+// 53, 4096 of 7168 89 / 84; 4097 of 2048 fp32 47 / 57, of 7168 153 / 184: fp32, whose sums take fewer registers, has six CTAs on an SM
+// without it (with four of them 58 us).
 template <typename T, int N, int U, int GROUP, bool AHEAD>
 __global__ void __launch_bounds__(kMoveThreads, AHEAD ? 4 : 6)
 unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restrict__ pos, const float* __restrict__ weights,
@@ -488,7 +503,7 @@ unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restr
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-              for (int i = 0; i < N; ++i) acc[u][i] = fmaf(weight[j], to_float(x[j][u].v[i]), acc[u][i]);
+              for (int i = 0; i < N; ++i) acc[u][i] = fmaf(weight[j], elem(x[j][u], i), acc[u][i]);
           }
         if (top_k <= kSumBatch) break;
         k0 = k0 + kSumBatch < top_k ? k0 + kSumBatch : 0;   // (more choices: the next eight, and the first again for the next v)
@@ -526,18 +541,18 @@ struct UnpermuteGrad {
   int top_k, row_vecs;
 };
 
-// One CTA per token: its row of dout is read once (top_k <= 8), each sorted row of y read and of dy written once; the dots are
-// summed by shuffles and over the four warps in a fixed order.
-template <typename T, int N, int U>
+// A GROUP of threads per token: its row of dout is read once (top_k <= 8), each sorted row of y read and of dy written once; the
+// dots are summed by shuffles and over the group's warps in a fixed order.
+template <typename T, int N, int U, int GROUP>
 __global__ void __launch_bounds__(kMoveThreads, U > 1 ? 4 : 5)
 unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long items) {
   using P = Pack<T, N>;
-  constexpr int kWarps = kMoveThreads / 32;
+  constexpr int kWarps = GROUP / 32, kGroups = kMoveThreads / GROUP;
   __shared__ float s_dot[kWarps][kSumBatch];
   chain_wait();
   chain_release();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (long long t = blockIdx.x; t < items; t += gridDim.x) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32 % kWarps, thread = threadIdx.x % GROUP;
+  for (long long t = (long long)blockIdx.x * kGroups + threadIdx.x / GROUP; t < items; t += (long long)gridDim.x * kGroups) {
     if (t >= p.tokens) {
       zero_empty_rows<P>(p.pair, p.used_rows, p.rows, 1, reinterpret_cast<uint8_t*>(p.dy), p.dy_stride * (long long)sizeof(T),
                          p.row_vecs, (t - p.tokens) * kWarps + warp, lane);
@@ -554,15 +569,15 @@ unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long item
         wt[j] = there && p.weights ? p.weights[t * p.w_stride + k0 + j] : 1.f;
         dot[j] = 0.f;
       }
-      for (int v = threadIdx.x; v < p.row_vecs; v += U * kMoveThreads) {
+      for (int v = thread; v < p.row_vecs; v += U * GROUP) {
         // (loads behind the end repeat the last vector; neither stored nor summed)
         int at[U];
         bool there[U];
         P d[U], x[kSumBatch][U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          at[u] = U == 1 ? v : min(v + u * kMoveThreads, p.row_vecs - 1);
-          there[u] = U == 1 || v + u * kMoveThreads < p.row_vecs;
+          at[u] = U == 1 ? v : min(v + u * GROUP, p.row_vecs - 1);
+          there[u] = U == 1 || v + u * GROUP < p.row_vecs;
           d[u] = load_pack(dout + at[u]);
         }
         if (p.dw) {
@@ -580,31 +595,35 @@ unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long item
           for (int u = 0; u < U; ++u) {
             if (p.dw && there[u]) {
 #pragma unroll
-              for (int i = 0; i < N; ++i) dot[j] = fmaf(to_float(d[u].v[i]), to_float(x[j][u].v[i]), dot[j]);
+              for (int i = 0; i < N; ++i) dot[j] = fmaf(elem(d[u], i), elem(x[j][u], i), dot[j]);
             }
             if (p.dy && there[u]) {
               P r;
 #pragma unroll
-              for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(wt[j] * to_float(d[u].v[i]));
+              for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(wt[j] * elem(d[u], i));
               store_pack(reinterpret_cast<P*>(p.dy + row[j] * p.dy_stride) + at[u], r);
             }
           }
         }
       }
       if (p.dw) {
+        float* dw = p.dw + t * p.top_k + k0;
 #pragma unroll
         for (int j = 0; j < kSumBatch; ++j) {
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
-          if (lane == 0) s_dot[warp][j] = dot[j];
+          if (kWarps > 1 && lane == 0) s_dot[warp][j] = dot[j];
+          if (kWarps == 1 && lane == j && k0 + j < p.top_k) dw[j] = dot[j];
         }
-        __syncthreads();
-        if (threadIdx.x < kSumBatch && k0 + threadIdx.x < p.top_k) {
-          float sum = 0.f;
-          for (int w = 0; w < kWarps; ++w) sum += s_dot[w][threadIdx.x];
-          p.dw[t * p.top_k + k0 + threadIdx.x] = sum;
+        if (kWarps > 1) {
+          __syncthreads();
+          if (thread < kSumBatch && k0 + thread < p.top_k) {
+            float sum = 0.f;
+            for (int w = 0; w < kWarps; ++w) sum += s_dot[w][thread];
+            dw[thread] = sum;
+          }
+          __syncthreads();
         }
-        __syncthreads();
       }
     }
   }
@@ -670,16 +689,26 @@ cudaError_t unpermute_type(const void* y, long long y_stride, const int* pos, co
   return go(y, y_stride, pos, weights, w_stride, out, out_stride, tokens, top_k, hidden, num_sms, stream);
 }
 
-template <typename T, int N>
-cudaError_t launch_unpermute_grad(UnpermuteGrad<T> p, int hidden, int num_sms, cudaStream_t stream) {
-  p.row_vecs = hidden / N;
-  constexpr int kWarps = kMoveThreads / 32;
+template <typename T, int N, int U, int GROUP>
+cudaError_t launch_unpermute_grad_group(const UnpermuteGrad<T>& p, int num_sms, cudaStream_t stream) {
+  constexpr int kWarps = GROUP / 32, kGroups = kMoveThreads / GROUP;
   const long long items = p.tokens + (p.dy ? (p.rows + kZeroRows * kWarps - 1) / (kZeroRows * kWarps) : 0);
   if (items == 0) return cudaSuccess;
+  return launch_chained(unpermute_grad_kernel<T, N, U, GROUP>, dim3(grid_for((items + kGroups - 1) / kGroups, 64ll * num_sms)),
+                        dim3(kMoveThreads), 0, stream, p, items);
+}
+
+template <typename T, int N>
+cudaError_t launch_unpermute_grad(UnpermuteGrad<T> p, int hidden, int num_sms, cudaStream_t stream) {
   // single elements: more loads in flight.  us, one at a time / four: 2048 tokens x 8 of 4097 bf16 104 / 80, fp32 132 / 108; pairs of
   // 16-bit elements gain nothing
   constexpr int U = N == 1 ? 4 : 1;
-  return launch_chained(unpermute_grad_kernel<T, N, U>, dim3(grid_for(items, 64ll * num_sms)), dim3(kMoveThreads), 0, stream, p, items);
+  p.row_vecs = hidden / N;
+  // Many short rows by single warps.  us, groups of 32 / of 128, eight choices: bf16 16384 tokens of 512 71 / 98, 8192 of 1024 64 / 62,
+  // 4097 of 601 21 / 31, 100 of 2048 16 / 5 (with elements one by one, see elem); fp32 16384 of 256 51 / 70, 8192 of 1024 93 / 88.
+  const bool small = p.row_vecs < (U > 1 ? 2 : 1) * U * kMoveThreads && p.tokens >= 4ll * num_sms;
+  return small ? launch_unpermute_grad_group<T, N, U, 32>(p, num_sms, stream)
+               : launch_unpermute_grad_group<T, N, U, kMoveThreads>(p, num_sms, stream);
 }
 
 template <typename T>

@@ -33,7 +33,7 @@ def check(x, x_cpu=None, **kw):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 7168), (3, 128), (63, 129), (64, 256), (65, 127), (200, 1000), (130, 8)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 7168), (3, 128), (63, 129), (64, 256), (65, 127), (200, 1000), (130, 8), (35, 1100), (300, 600), (17, 2048)])
 @pytest.mark.parametrize("layout", ["kt", "tk"])
 def test_codes_and_scales_are_the_formulas(dtype, rows, cols, layout):
     g = torch.Generator().manual_seed(rows * 1000 + cols)

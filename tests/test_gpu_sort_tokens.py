@@ -104,7 +104,7 @@ def sums(y, pos, w):
 
 SIZES = [(1, 7168, 8, 256, 256, 1), (7, 1, 2, 16, 16, 4), (50, 129, 8, 64, 16, 16), (301, 520, 6, 64, 64, 128), (64, 2048, 32, 40, 40, 1),
          (1200, 72, 1, 8, 8, 1), (10, 1031, 9, 30, 30, 1), (20, 1602, 10, 30, 30, 1), (700, 4097, 8, 64, 64, 1), (3000, 514, 3, 16, 12, 1),
-         (5000, 250, 9, 16, 16, 1)]
+         (5000, 250, 9, 16, 16, 1), (1100, 320, 3, 16, 16, 8)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
