@@ -6,12 +6,12 @@
 // memory from zero, read back and folded into fp32 registers with one FMA each, the factor being one number per row (= TMEM
 // lane = thread) and 128-column slab.
 //
-// Two kernels: 128 x 128 tiles, two CTAs on an SM, the K blocks of a tile divided over a cluster where tiles are few; and
-// 256 x 256 tiles of a CTA pair (cta_group::2) where there are enough of them.
+// Two kernels: 128 x 128 tiles, one CTA on an SM with four accumulators or two with two each, the K blocks of a tile divided over a
+// cluster where tiles are few; and 256 x 256 tiles of a CTA pair (cta_group::2) where there are enough of them.
 //
-// Few rows are bound by the weights' bytes and, below some 30 MB of them, by latency: one row through 4096 x 7168 takes 8.8 us (29
-// MB, 4.5 us at the copy rate), through 7168 x 16384 23.9 us (117 MB, 17.9).  Many rows are bound by the hand-offs between tensor
-// cores and promotion: 8192 x 4096 x 7168 takes 229 us, 2.1 PFLOP/s, some 1000 cycles for a K block of a tile whose MMAs take 512.
+// Few rows are bound by the weights' bytes and, below some 30 MB of them, by latency: one row through 4096 x 7168 takes 9.4 us (29
+// MB, 4.5 us at the copy rate), through 7168 x 16384 24.6 us (117 MB, 17.9).  Many rows are bound by the hand-offs between tensor
+// cores and promotion: 8192 x 4096 x 7168 takes 222 us, 2.2 PFLOP/s, some 1000 cycles for a K block of a tile whose MMAs take 512.
 // An accumulator's way round - issue 200 cycles, MMAs 260 to 510, the look at the barrier 200 to 300, read-back 250 to 300, the
 // counter's way back 200 and more - is longer than the MMAs of the other one, and tensor memory has no room for a third.
 #include "common.cuh"
@@ -343,11 +343,13 @@ __device__ __forceinline__ void report_status(const MatmulParams& p, const int* 
 // ------------------------------ 128 x 128 tiles ------------------------------
 
 constexpr int kMidThreads = 256;                 // warps 0: TMA, 1-2: MMA issuers, 3: scales, 4-7: promotion and epilogue
-constexpr int kMidStages = 3;
-constexpr int kMidAcc = 2;                       // accumulators in tensor memory
-constexpr int kMidSmemBytes = kMidStages * kStageBytes + kScaleRing * kTile * 4 + 1024;
-static_assert(kMidStages >= kMidAcc + 1, "what an issuer knows of a stage's use before (see there)");
-static_assert(kMidStages * kStageBytes >= 3 * 11 * kTile * 16, "the join of a split product (three parts of eleven vectors are most) reuses the ring");
+// ACC accumulators in tensor memory: two, with three stages, where CTAs share an SM; four, with six, where each has one alone (a K
+// block then takes 300 ns instead of 360: more of its way round runs beside the others').
+constexpr int mid_stages(int acc) { return acc == 2 ? 3 : 6; }
+constexpr int mid_smem_bytes(int acc) { return mid_stages(acc) * kStageBytes + kScaleRing * kTile * 4 + 1024; }
+static_assert(mid_stages(2) >= 2 && mid_stages(4) >= 4, "what an issuer knows of a stage's use before (see there)");
+static_assert(mid_stages(2) * kStageBytes >= 3 * 11 * kTile * 16,
+              "the join of a split product (three parts of eleven vectors are most) reuses the ring");
 // setmaxnreg moves registers inside what the CTA was launched with (256 threads x 128): the four control warps give up
 // 128 x (128 - 48), the four promotion warps take 128 x (208 - 128).
 constexpr int kMidLaunchRegs = 128, kMidCtrlRegs = 48, kMidPromoRegs = 208;
@@ -395,30 +397,32 @@ __device__ __forceinline__ void join_split(const MatmulParams& p, const float2* 
   }
 }
 
+template <int ACC>
 __global__ void __launch_bounds__(kMidThreads, 2)
 block_matmul_kernel(const __grid_constant__ MatmulParams p) {
+  constexpr int kStages = mid_stages(ACC);
   const int split = p.split;
   const int tile = blockIdx.x / split, part = blockIdx.x % split;
   const int m0 = tile % p.m_tiles * kTile, n0 = tile / p.m_tiles * kTile;
   const int rows = min(kTile, p.M - m0), promo_warps = (rows + 31) / 32;   // (warps without a row only take part in the barriers)
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t s_bars[2 * kMidStages + kMidAcc + 2 + 2 * kScaleRing];
-  __shared__ uint32_t s_read[kMidAcc];
+  __shared__ uint64_t s_bars[2 * kStages + ACC + 2 + 2 * kScaleRing];
+  __shared__ uint32_t s_read[ACC];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort[2], s_status[2];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t bar_full = smem_u32(s_bars), bar_empty = bar_full + 8 * kMidStages;
-  const uint32_t bar_done = bar_empty + 8 * kMidStages, bar_drain = bar_done + 8 * kMidAcc, count_read = smem_u32(s_read);
+  const uint32_t bar_full = smem_u32(s_bars), bar_empty = bar_full + 8 * kStages;
+  const uint32_t bar_done = bar_empty + 8 * kStages, bar_drain = bar_done + 8 * ACC, count_read = smem_u32(s_read);
   const uint32_t bar_factors = bar_drain + 16, bar_slot = bar_factors + 8 * kScaleRing;   // a factor slot is filled, is free
   volatile int* abort_flag = s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kMidStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
     }
-    for (int b = 0; b < kMidAcc; ++b) {
+    for (int b = 0; b < ACC; ++b) {
       mbar_init(bar_done + 8 * b, 1);
       s_read[b] = 0;
     }
@@ -435,7 +439,7 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
     tma_prefetch_desc(&p.tmap_b);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(&s_tmem), kMidAcc * kTile);
+    tmem_alloc(smem_u32(&s_tmem), ACC * kTile);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -445,7 +449,7 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
 
   const int kb0 = (int)((long long)p.kblocks * part / split), kb1 = (int)((long long)p.kblocks * (part + 1) / split);
   const int steps = kb1 - kb0;
-  const uint32_t factors = smem_base + kMidStages * kStageBytes;
+  const uint32_t factors = smem_base + kStages * kStageBytes;
   chain_wait();
   chain_release();
 
@@ -454,34 +458,34 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
     if (warp == 0 && lane == 0) {
       int it = 0;
       for (; it < steps; ++it) {
-        const int s = it % kMidStages;
-        if (!mbar_poll(bar_empty + 8 * s, ((it / kMidStages) & 1) ^ 1, abort_flag, s_status, 1)) break;
+        const int s = it % kStages;
+        if (!mbar_poll(bar_empty + 8 * s, ((it / kStages) & 1) ^ 1, abort_flag, s_status, 1)) break;
         mbar_arrive_expect_tx(bar_full + 8 * s, kOperandBytes + p.box_rows * kBlockK);
         const uint32_t dst = smem_base + s * kStageBytes;
         tma_load_2d(dst + kOperandBytes, &p.tmap_b, (kb0 + it) * kBlockK, n0, bar_full + 8 * s);
         tma_load_2d(dst, &p.tmap_a, (kb0 + it) * kBlockK, m0, bar_full + 8 * s);
       }
       // copies still in flight must land before the ring is used otherwise or released
-      for (int j = it > kMidStages ? it - kMidStages : 0; j < it; ++j)
-        (void)mbar_poll(bar_full + 8 * (j % kMidStages), (j / kMidStages) & 1, abort_flag + 1, s_status, 2);
+      for (int j = it > kStages ? it - kStages : 0; j < it; ++j)
+        (void)mbar_poll(bar_full + 8 * (j % kStages), (j / kStages) & 1, abort_flag + 1, s_status, 2);
     } else if (warp == 1 || warp == 2) {
-      // Two issuers take turns, each with an accumulator of its own: a turn takes some 700 cycles, an MMA chain's 256.  The whole
+      // Two issuers take turns, each with accumulators of its own: a turn takes some 700 cycles, an MMA chain's 256.  The whole
       // warp runs the loop and one elected lane issues (a lane of its own took 450 cycles for four MMAs and two commits, this
-      // 330 and less).  The stage's barrier is looked at only once K block it - 2 has been read back, which says that the stage's
-      // use before, K block it - 3 of the other issuer, has landed: a parity is not to be asked about two phases ahead.
+      // 330 and less).  The stage's barrier is looked at only once K block it - ACC has been read back, and with it all before:
+      // so the stage's use before, K block it - kStages, has landed.  A parity is not to be asked about two phases ahead.
       constexpr uint32_t idesc = make_idesc_e4m3(kTile, kTile);
       const int me = warp - 1;
-      for (int it = me; it < steps; it += kMidAcc) {
-        const int s = it % kMidStages;
-        bool ok = count_poll(count_read + 4 * me, promo_warps * (it / kMidAcc), abort_flag, s_status, 3);
-        ok = ok && mbar_poll(bar_full + 8 * s, (it / kMidStages) & 1, abort_flag, s_status, 4);
+      for (int it = me; it < steps; it += 2) {
+        const int s = it % kStages, b = it % ACC;
+        bool ok = count_poll(count_read + 4 * b, promo_warps * (it / ACC), abort_flag, s_status, 3);
+        ok = ok && mbar_poll(bar_full + 8 * s, (it / kStages) & 1, abort_flag, s_status, 4);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t a_addr = smem_base + s * kStageBytes;
         if (elect_one()) {
-          tc_mma_f8_kblock(tmem + me * kTile, kmajor_sw128_desc_lo(a_addr), kmajor_sw128_desc_lo(a_addr + kOperandBytes),
+          tc_mma_f8_kblock(tmem + b * kTile, kmajor_sw128_desc_lo(a_addr), kmajor_sw128_desc_lo(a_addr + kOperandBytes),
                            kKmajorSw128DescHi, idesc);
-          tc_commit(bar_done + 8 * me);
+          tc_commit(bar_done + 8 * b);
           tc_commit(bar_empty + 8 * s);
         }
         __syncwarp();
@@ -510,10 +514,10 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
     for (int j = 0; j < kTile / 2; ++j) acc[j] = make_float2(0.f, 0.f);
     uint32_t seen_f = 0, seen_d = 0;   // the coming K block's factors, accumulator are known to be there (looked at below)
     for (int it = 0; it < steps && warp - 4 < promo_warps; ++it) {
-      const int b = it % kMidAcc;
+      const int b = it % ACC;
       if (!(seen_f & seen_d)) {
         const bool ok = (seen_f || mbar_poll(bar_factors + 8 * (it % kScaleRing), (it / kScaleRing) & 1, abort_flag, s_status, 8)) &&
-                        (seen_d || mbar_wait(bar_done + 8 * b, (it / kMidAcc) & 1, abort_flag, s_status, 6));
+                        (seen_d || mbar_wait(bar_done + 8 * b, (it / ACC) & 1, abort_flag, s_status, 6));
         if (!__all_sync(0xffffffffu, ok)) break;
       }
       tc_fence_after();
@@ -525,7 +529,7 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
         }
         const uint32_t n = it + 1;
         seen_f = mbar_test_wait(bar_factors + 8 * (n % kScaleRing), (n / kScaleRing) & 1);
-        seen_d = mbar_test_wait(bar_done + 8 * (n % kMidAcc), (n / kMidAcc) & 1);
+        seen_d = mbar_test_wait(bar_done + 8 * (n % ACC), (n / ACC) & 1);
       });
       seen_f = __all_sync(0xffffffffu, seen_f);
       seen_d = __all_sync(0xffffffffu, seen_d);
@@ -548,7 +552,7 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, kMidAcc * kTile);
+  if (warp == 1) tmem_dealloc(tmem, ACC * kTile);
   if (threadIdx.x == 0) report_status(p, s_abort, s_status);
 }
 
@@ -798,32 +802,40 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
   if (threadIdx.x == 0) report_status(p, s_abort, s_status);
 }
 
-// What a call takes, in ns, by a fit to measured times (us, bf16 results, weights of 7 to 117 MB):
-// 128 x 128 tiles with S parts of K.  A K block takes 360 ns where an SM has one CTA, 590 where it has two; the join's time goes
-// with the rows that travel.  N 4096, K 7168: 1 row S 1 23.1, 2 14.3, 4 9.7, 8 8.8; 128 rows 26.0, 18.5, 13.8, 17.3; 300 rows 26.5,
-// 24.5, 30.4, 41.3.  N 7168, K 2048: 1 row 9.0, 7.0, 6.6, 10.8; 128 rows 10.6, 10.8, 12.8, 23.6.  N 7168, K 16384: 128 rows 56.4, 36.8,
-// 31.1, 42.5; 300 rows 71.3, 77.5, 71.6, 94.1.  A cluster's CTAs have to be neighbours: of clusters of three not all places
-// can be had (288 CTAs 29.9 instead of 24.5), singly on an SM seven eighths of any.
-long long mid_cost(long long tiles, int kblocks, int rows, int S, int num_sms) {
-  const long long ctas = tiles * S, wave = S == 3 ? num_sms * 7 / 4 : 2 * num_sms, full = ctas / wave, rest = ctas - full * wave;
-  const long long steps = (kblocks + S - 1) / S;
-  const long long one = steps * 360 + (S == 1 ? 300 : 400 + rows * (2300 + 250 * S) / kTile);
-  const long long two = steps * 590 + (S == 1 ? 300 : 600 + rows * (800 + 1000 * S) / kTile);
-  // (from the third wave on L2 has 13 TB/s to deliver)
-  return (full >= 2 ? full * two * 9 / 8 : full * two) + (rest == 0 ? 0 : rest <= (S == 1 ? num_sms : num_sms * 7 / 8) ? one : two);
+// Whether every CTA of 128 x 128 tiles with S parts of K has an SM alone.  A cluster's CTAs have to be neighbours, for which not
+// all places can be had.
+bool mid_alone(long long ctas, int S, int num_sms) { return ctas <= (S == 1 ? num_sms : num_sms * 7 / 8); }
+
+// What a call takes, in ns and less what all take, by a fit to measured times (us, bf16 results, weights of 7 to 117 MB).
+// 128 x 128 tiles with S parts of K.  A K block takes 300 ns where CTAs have an SM alone (360 in the last wave of several), 590 where two
+// share it; the join's time goes with the rows that travel.  S 1, 2, 3, 4, 8; *: shared SMs.  N 4096, K 7168: 1 row 19.3, 12.3, 10.2,
+// 9.4, 9.3*; 128 rows 20.9, 16.0, 14.1, 12.9, 17.0*; 300 rows 21.7, 23.3*, 28.9*, 29.3*, 40.5*.  N 7168, K 2048: 1 row 7.9, 6.9, 7.2*, 7.0*, 11.1*;
+// 128 rows 8.6, 10.1, 12.9*, 12.8*, 23.9*.  N 7168, K 16384: 128 rows 45.9, 30.5, 33.2*, 29.8*, 42.4*; 300 rows 69.6*, 74.2*, 59.9*, 68.9*, 91.0*.
+// Of several waves each costs CTAs' coming and going too, and from the third on L2's rate: see below.  `rough`: rows of A or B do not
+// start on sectors (32 bytes), so that a tile's row is five of them.  512 x 6016 x 1504 11.4, x 1488 14.4; 1536 x 1536 x 7136 22.1,
+// x 7152 26.3; 8000 x 1536 x 2080 39, x 2064 51 (pairs 32.3, 33.4).
+long long mid_cost(long long tiles, int kblocks, int rows, int S, bool rough, int num_sms) {
+  const long long ctas = tiles * S, steps = (kblocks + S - 1) / S, shared = rough ? 860 : 590;
+  const long long join = S == 1 ? 300 : 400 + rows * (2300 + 250 * S) / kTile, join2 = S == 1 ? 300 : 600 + rows * (800 + 1000 * S) / kTile;
+  if (mid_alone(ctas, S, num_sms)) return steps * (285 + (rough ? 135 : 60) * rows / kTile) + join;
+  const long long wave = S == 3 ? num_sms * 7 / 4 : 2 * num_sms, full = ctas / wave, rest = ctas - full * wave;
+  const long long last = rest == 0 ? 0 : mid_alone(rest, S, num_sms) ? steps * 360 + join : steps * shared + join2;
+  return full * (steps * (full >= 2 ? shared + 30 : shared) + join2 + (full >= 2 ? 2700 : 2200)) + last + (full ? 1000 : 0);
 }
-// 256 x 256 tiles, one pair of SMs each.  M x 1536 x 7168, 128 x 128 tiles / pairs: M 1536 23.1 / 31.0, 2048 32.9 / 32.3, 4096 54.6 /
-// 59.5; M x 4096 x 7168: 640 32.7 / 32.8, 1024 33.3 / 32.0, 1536 54.8 / 59.7, 2048 65.8 / 59.7, 3000 104.7 / 88.5, 8192 274 / 228;
-// M x 7168 x 16384: 1024 146 / 130, 2048 300 / 261, 4096 575 / 530.
+// 256 x 256 tiles, one pair of SMs each.  128 x 128 tiles / pairs: M x 1536 x 7168: M 1536 21.9 / 31.0, 2048 32.9 / 30.8, 4096 54.6 / 59.5; M x
+// 4096 x 7168: 640 32.7 / 30.9, 1024 33.3 / 30.7, 1536 54.8 / 59.7, 2048 65.8 / 59.7, 3000 104.7 / 88.5, 8192 274 / 225; M x 7168 x 16384: 1024
+// 146 / 130, 2048 300 / 261, 4096 575 / 530; 2124 x 2190 x 6352 68 / 50, 3709 x 4480 x 1264 42 / 30, 2138 x 4608 x 704 19 / 17.
 long long pair_cost(long long tiles, int kblocks, int num_sms) {
   const long long pairs = num_sms / 2;
-  return (tiles + pairs - 1) / pairs * (kblocks * 530ll + 1000);
+  return (tiles + pairs - 1) / pairs * (kblocks * 530ll + 1500);
 }
 
 }  // namespace
 
 cudaError_t configure_block_matmul() {
-  cudaError_t e = cudaFuncSetAttribute(block_matmul_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMidSmemBytes);
+  cudaError_t e = cudaFuncSetAttribute(block_matmul_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, mid_smem_bytes(2));
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(block_matmul_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, mid_smem_bytes(4));
   if (e != cudaSuccess) return e;
   return cudaFuncSetAttribute(block_matmul_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes);
 }
@@ -869,11 +881,13 @@ extern "C" int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride, cons
   p.status = status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 
+  const int rows = M < kTile ? M : kTile;
+  const bool rough = (a_row_stride | b_row_stride) % 32 != 0;
   p.split = 1;
-  long long cost = mid_cost(m_tiles * n_tiles, p.kblocks, M < kTile ? M : kTile, 1, num_sms);
+  long long cost = mid_cost(m_tiles * n_tiles, p.kblocks, rows, 1, rough, num_sms);
   for (int S : {2, 3, 4, 8}) {
     if (2 * S > p.kblocks) break;
-    const long long c = mid_cost(m_tiles * n_tiles, p.kblocks, M < kTile ? M : kTile, S, num_sms);
+    const long long c = mid_cost(m_tiles * n_tiles, p.kblocks, rows, S, rough, num_sms);
     if (c < cost) {
       cost = c;
       p.split = S;
@@ -893,11 +907,13 @@ extern "C" int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride, cons
   }
   if ((rc = make_tmap(&p.tmap_b, b, (uint64_t)N, (uint64_t)K, (uint64_t)b_row_stride, kTile)) != B200MOE_OK) return rc;
   // fewer rows than a tile has are a smaller copy
-  p.box_rows = M < kTile ? M : kTile;
+  p.box_rows = rows;
   if ((rc = make_tmap(&p.tmap_a, a, (uint64_t)M, (uint64_t)K, (uint64_t)a_row_stride, (uint32_t)p.box_rows)) != B200MOE_OK) return rc;
   p.m_tiles = (int)m_tiles;
   p.n_tiles = (int)n_tiles;
-  CUDA_TRY(launch_chained_cluster(block_matmul_kernel, dim3((unsigned)(m_tiles * n_tiles * p.split)), dim3(kMidThreads), kMidSmemBytes,
-                                  st, p.split, p));
+  const long long ctas = m_tiles * n_tiles * p.split;
+  const bool alone = mid_alone(ctas, p.split, num_sms);
+  CUDA_TRY(launch_chained_cluster(alone ? block_matmul_kernel<4> : block_matmul_kernel<2>, dim3((unsigned)ctas), dim3(kMidThreads),
+                                  mid_smem_bytes(alone ? 4 : 2), st, p.split, p));
   return B200MOE_OK;
 }
