@@ -336,16 +336,15 @@ struct RowMove {
 };
 
 constexpr int kMoveThreads = 128;
-constexpr int kZeroRows = 4;                     // sorted rows that a warp looks at for empty ones
 
-// Rows of `dst` without a pair become zero; `item` counts groups of kZeroRows rows.
+// Rows of `dst` without a pair become zero; `item` counts groups of `zero_rows` (at most 32) rows.
 template <typename V>
 __device__ __forceinline__ void zero_empty_rows(const int* pair, const int* used_rows, long long rows, int zero_tail, uint8_t* dst,
-                                                long long dst_stride, int row_vecs, long long item, int lane) {
-  const long long r0 = item * kZeroRows;
+                                                long long dst_stride, int row_vecs, int zero_rows, long long item, int lane) {
+  const long long r0 = item * zero_rows;
   const long long limit = zero_tail ? rows : (long long)*used_rows;
   bool empty = false;
-  if (lane < kZeroRows && r0 + lane < rows && r0 + lane < limit) empty = pair[r0 + lane] < 0;
+  if (lane < zero_rows && r0 + lane < rows && r0 + lane < limit) empty = pair[r0 + lane] < 0;
   unsigned todo = __ballot_sync(0xffffffffu, empty);
   while (todo) {
     const int j = __ffs(todo) - 1;
@@ -355,34 +354,40 @@ __device__ __forceinline__ void zero_empty_rows(const int* pair, const int* used
   }
 }
 
-// A warp takes U x 32 vectors of one token's row into registers and stores them to the token's sorted rows.
+// Sorted rows that a warp looks at for empty ones: some 28 KB, so that those that are empty do not make a warp's work much longer than
+// a token's, and a look without one is a small part of what it goes with.
+int zero_rows_of(long long row_bytes) { return (int)(row_bytes >= 28672 ? 1 : row_bytes * 32 <= 28672 ? 32 : 28672 / row_bytes); }
+
+// A warp takes U x 32 vectors of one token's row into registers and stores them to the token's sorted rows, or looks at sorted rows
+// for empty ones.  One small piece of work a warp, and as many CTAs as that takes: 4096 tokens of 14 KB to 65280 rows of which half are
+// empty take 153 us (6.5 TB/s); with four rows to look at, 512 bytes of a token and 64 CTAs an SM that took several pieces each, 174.
 template <typename V, int U>
 __global__ void __launch_bounds__(kMoveThreads)
-permute_kernel(const __grid_constant__ RowMove p, int segments, long long move_items, long long items) {
+permute_kernel(const __grid_constant__ RowMove p, int segments, int segment_vecs, int zero_rows, long long move_items, long long items) {
   chain_wait();
   chain_release();
   const int lane = threadIdx.x & 31;
   const long long step = (long long)gridDim.x * (kMoveThreads / 32);
   for (long long w = (long long)blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); w < items; w += step) {
     if (w >= move_items) {
-      zero_empty_rows<V>(p.pair, p.used_rows, p.rows, p.zero_tail, p.dst, p.dst_stride, p.row_vecs, w - move_items, lane);
+      zero_empty_rows<V>(p.pair, p.used_rows, p.rows, p.zero_tail, p.dst, p.dst_stride, p.row_vecs, zero_rows, w - move_items, lane);
       continue;
     }
     const long long t = w / segments;
-    const int v0 = (int)(w - t * segments) * (U * 32) + lane;
+    const int v_begin = (int)(w - t * segments) * segment_vecs, v_end = min(v_begin + segment_vecs, p.row_vecs), v0 = v_begin + lane;
     const int mine = lane < p.top_k ? p.pos[t * p.top_k + lane] : -1;
     const V* src = reinterpret_cast<const V*>(p.src + t * p.src_stride);
     V x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (v0 + u * 32 < p.row_vecs) x[u] = __ldg(src + v0 + u * 32);
+      if (v0 + u * 32 < v_end) x[u] = __ldg(src + v0 + u * 32);
     for (int k = 0; k < p.top_k; ++k) {
       const int row = __shfl_sync(0xffffffffu, mine, k);
       if (row < 0) continue;
       V* dst = reinterpret_cast<V*>(p.dst + row * p.dst_stride);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (v0 + u * 32 < p.row_vecs) dst[v0 + u * 32] = x[u];
+        if (v0 + u * 32 < v_end) dst[v0 + u * 32] = x[u];
     }
   }
 }
@@ -545,7 +550,7 @@ struct UnpermuteGrad {
 // dots are summed by shuffles and over the group's warps in a fixed order.
 template <typename T, int N, int U, int GROUP>
 __global__ void __launch_bounds__(kMoveThreads, U > 1 ? 4 : 5)
-unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long items) {
+unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, int zero_rows, long long items) {
   using P = Pack<T, N>;
   constexpr int kWarps = GROUP / 32, kGroups = kMoveThreads / GROUP;
   __shared__ float s_dot[kWarps][kSumBatch];
@@ -555,7 +560,7 @@ unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long item
   for (long long t = (long long)blockIdx.x * kGroups + threadIdx.x / GROUP; t < items; t += (long long)gridDim.x * kGroups) {
     if (t >= p.tokens) {
       zero_empty_rows<P>(p.pair, p.used_rows, p.rows, 1, reinterpret_cast<uint8_t*>(p.dy), p.dy_stride * (long long)sizeof(T),
-                         p.row_vecs, (t - p.tokens) * kWarps + warp, lane);
+                         p.row_vecs, zero_rows, (t - p.tokens) * kWarps + warp, lane);
       continue;
     }
     const P* dout = reinterpret_cast<const P*>(p.dout + t * p.dout_stride);
@@ -632,13 +637,14 @@ unpermute_grad_kernel(const __grid_constant__ UnpermuteGrad<T> p, long long item
 unsigned grid_for(long long items, long long most) { return (unsigned)(items < most ? items : most); }
 
 template <typename V, int U>
-cudaError_t launch_permute_rows(const RowMove& p, int num_sms, cudaStream_t stream) {
-  const int segments = (p.row_vecs + U * 32 - 1) / (U * 32);
+cudaError_t launch_permute_rows(const RowMove& p, cudaStream_t stream) {
+  const int pieces = (p.row_vecs + 31) / 32, segments = (pieces + U - 1) / U, segment_vecs = (pieces + segments - 1) / segments * 32;
+  const int zero_rows = zero_rows_of((long long)p.row_vecs * (long long)sizeof(V));
   const long long move_items = p.tokens * segments;
-  const long long items = move_items + (p.rows + kZeroRows - 1) / kZeroRows;
+  const long long items = move_items + (p.rows + zero_rows - 1) / zero_rows;
   constexpr int kWarps = kMoveThreads / 32;
-  return launch_chained(permute_kernel<V, U>, dim3(grid_for((items + kWarps - 1) / kWarps, 64ll * num_sms)), dim3(kMoveThreads), 0,
-                        stream, p, segments, move_items, items);
+  return launch_chained(permute_kernel<V, U>, dim3(grid_for((items + kWarps - 1) / kWarps, 0x7fffffffll)), dim3(kMoveThreads), 0, stream, p,
+                        segments, segment_vecs, zero_rows, move_items, items);
 }
 
 template <typename T, int N, int U, int GROUP>
@@ -692,10 +698,11 @@ cudaError_t unpermute_type(const void* y, long long y_stride, const int* pos, co
 template <typename T, int N, int U, int GROUP>
 cudaError_t launch_unpermute_grad_group(const UnpermuteGrad<T>& p, int num_sms, cudaStream_t stream) {
   constexpr int kWarps = GROUP / 32, kGroups = kMoveThreads / GROUP;
-  const long long items = p.tokens + (p.dy ? (p.rows + kZeroRows * kWarps - 1) / (kZeroRows * kWarps) : 0);
+  const int zero_rows = zero_rows_of((long long)p.row_vecs * N * (long long)sizeof(T));
+  const long long items = p.tokens + (p.dy ? (p.rows + zero_rows * kWarps - 1) / (zero_rows * kWarps) : 0);
   if (items == 0) return cudaSuccess;
   return launch_chained(unpermute_grad_kernel<T, N, U, GROUP>, dim3(grid_for((items + kGroups - 1) / kGroups, 64ll * num_sms)),
-                        dim3(kMoveThreads), 0, stream, p, items);
+                        dim3(kMoveThreads), 0, stream, p, zero_rows, items);
 }
 
 template <typename T, int N>
@@ -705,8 +712,9 @@ cudaError_t launch_unpermute_grad(UnpermuteGrad<T> p, int hidden, int num_sms, c
   constexpr int U = N == 1 ? 4 : 1;
   p.row_vecs = hidden / N;
   // Many short rows by single warps.  us, groups of 32 / of 128, eight choices: bf16 16384 tokens of 512 71 / 98, 8192 of 1024 64 / 62,
-  // 4097 of 601 21 / 31, 100 of 2048 16 / 5 (with elements one by one, see elem); fp32 16384 of 256 51 / 70, 8192 of 1024 93 / 88.
-  const bool small = p.row_vecs < (U > 1 ? 2 : 1) * U * kMoveThreads && p.tokens >= 4ll * num_sms;
+  // 4097 of 601 21 / 31, 100 of 2048 16 / 5 (with elements one by one, see elem); fp32 16384 of 256 51 / 70, of
+  // 512 with two choices 38 / 51, 8192 of 1024 93 / 88.
+  const bool small = p.row_vecs < (U > 1 ? 2 : 1) * U * kMoveThreads + (sizeof(T) == 4) && p.tokens >= 4ll * num_sms;
   return small ? launch_unpermute_grad_group<T, N, U, 32>(p, num_sms, stream)
                : launch_unpermute_grad_group<T, N, U, kMoveThreads>(p, num_sms, stream);
 }
@@ -854,13 +862,13 @@ int b200moe_permute_rows(const void* x, int64_t x_row_bytes, int64_t row_bytes, 
   const int vec = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
   p.row_vecs = (int)(row_bytes / vec);
   if (vec == 16)
-    CUDA_TRY((launch_permute_rows<uint4, 1>(p, num_sms, st)));
+    CUDA_TRY((launch_permute_rows<uint4, 2>(p, st)));
   else if (vec == 4)
-    CUDA_TRY((launch_permute_rows<uint32_t, 4>(p, num_sms, st)));
+    CUDA_TRY((launch_permute_rows<uint32_t, 4>(p, st)));
   else if (vec == 2)
-    CUDA_TRY((launch_permute_rows<uint16_t, 8>(p, num_sms, st)));
+    CUDA_TRY((launch_permute_rows<uint16_t, 8>(p, st)));
   else
-    CUDA_TRY((launch_permute_rows<uint8_t, 8>(p, num_sms, st)));
+    CUDA_TRY((launch_permute_rows<uint8_t, 8>(p, st)));
   return B200MOE_OK;
 }
 
