@@ -73,21 +73,24 @@ def _no_gradient(what: str) -> RuntimeError:
     return RuntimeError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
-def _rows2d(t: torch.Tensor, what: str) -> torch.Tensor:
-    """``t`` with unit inner stride and rows that do not overlap (a copy where it has not); extents that 32 bits hold."""
+def _matrix(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
+    """(``t``, rows, columns, row stride in elements) with unit inner stride and rows that do not overlap (a copy where ``t`` has not);
+    extents that 32 bits hold.  The stride of a single row is free: torch may say anything."""
     if t.dim() != 2:
         raise ValueError(f"{what} must be 2-D, got shape {tuple(t.shape)}")
-    if t.shape[0] > _INT_MAX or t.shape[1] > _INT_MAX:
+    rows, cols = t.shape
+    if rows > _INT_MAX or cols > _INT_MAX:
         raise ValueError(f"{what} must have at most {_INT_MAX} rows and columns, got shape {tuple(t.shape)}")
     if t.is_contiguous():
-        return t
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
+        return t, rows, cols, cols
+    s0, s1 = t.stride()
+    if (cols > 1 and s1 != 1) or (rows > 1 and s0 < cols):
+        return t.contiguous(), rows, cols, cols
+    return t, rows, cols, s0 if rows > 1 else cols
 
 
 def _pitch(t: torch.Tensor) -> int:
-    """Row stride in elements (that of a single row is free: torch may say anything)."""
+    """Row stride in elements of a result that was checked."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
@@ -120,8 +123,7 @@ def quantize(x: torch.Tensor, *, swiglu: bool = False, scale_layout: str = "kt")
         raise ValueError(f"scale_layout must be 'kt' or 'tk', got {scale_layout!r}")
     if x.requires_grad and torch.is_grad_enabled():
         raise _no_gradient("quantize")
-    x = _rows2d(x, "x")
-    rows, cols = x.shape
+    x, rows, cols, pitch = _matrix(x, "x")
     if swiglu:
         if cols % 2:
             raise ValueError(f"swiglu needs an even number of columns (gate half, up half), got {cols}")
@@ -133,7 +135,7 @@ def quantize(x: torch.Tensor, *, swiglu: bool = False, scale_layout: str = "kt")
     else:
         scale, stride_t, stride_kb = torch.empty(rows, blocks, dtype=torch.float32, device=dev), blocks, 1
     if rows and cols:
-        _call("b200moe_quantize", dev.index, x.data_ptr(), dt, _pitch(x), rows, cols, int(swiglu), codes.data_ptr(), cols,
+        _call("b200moe_quantize", dev.index, x.data_ptr(), dt, pitch, rows, cols, int(swiglu), codes.data_ptr(), cols,
               scale.data_ptr(), stride_t, stride_kb)
     return codes, scale
 
@@ -164,9 +166,9 @@ def _block_scale_strides(scale: torch.Tensor, rows: int, blocks: int, layout: st
         raise TypeError(f"{what} must be float32, got {scale.dtype}")
     if layout == "kt":
         if scale.shape == (blocks, rows):
-            return scale.stride()[::-1]
+            return (1, rows) if scale.is_contiguous() else scale.stride()[::-1]
     elif scale.shape == (rows, blocks):
-        return scale.stride()
+        return (blocks, 1) if scale.is_contiguous() else scale.stride()
     want = (blocks, rows) if layout == "kt" else (rows, blocks)
     raise ValueError(f"{what} has shape {tuple(scale.shape)}, expected {want} for scale_layout {layout!r}")
 
@@ -190,8 +192,7 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
         raise _no_gradient("block_matmul")
     if a.dtype not in _CODES or b.dtype not in _CODES:
         raise TypeError(f"a and b must be float8_e4m3fn (or its uint8 bit pattern), got {a.dtype} and {b.dtype}")
-    a = _rows2d(a, "a")
-    M, K = a.shape
+    a, M, K, a_pitch = _matrix(a, "a")
     if b.dim() != 2 or b.shape[1] != K:
         raise ValueError(f"b must be [N, {K}], got {tuple(b.shape)}")
     N = b.shape[0]
@@ -204,14 +205,15 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     blocks = -(-K // BLOCK)
     as_m, as_kb = _block_scale_strides(a_scale, M, blocks, scale_layout, "a_scale")
     bs_n, bs_kb = _block_scale_strides(b_scale, -(-N // BLOCK), blocks, "tk", "b_scale")
-    a_ptr, a_pitch, b_ptr, b_pitch = a.data_ptr(), _pitch(a), b.data_ptr(), _pitch(b)
+    a_ptr, b_ptr = a.data_ptr(), b.data_ptr()
+    b_pitch = K if N == 1 or b.is_contiguous() else b.stride(0)
     if (b_ptr | b_pitch) % 16 or b_pitch < K or b.stride(1) != 1:
         raise ValueError("b must have unit inner stride and rows on 16-byte boundaries")
     if (a_ptr | a_pitch) % 16:
         a = a.clone(memory_format=torch.contiguous_format)
         a_ptr, a_pitch = a.data_ptr(), K
     if out is None:
-        dt = _DTYPE.get(out_dtype)
+        dt, out_pitch = _DTYPE.get(out_dtype), N
         if dt is None:
             raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
         out = torch.empty(M, N, dtype=out_dtype, device=dev)
@@ -220,6 +222,7 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
         if dt is None:
             raise TypeError(f"out must be float32, bfloat16 or float16, got {out.dtype}")
         _check_out(out, (M, N), out.dtype, dev)
+        out_pitch = _pitch(out)
     if M == 0 or N == 0:
         return out
     st = _status.get(dev.index)
@@ -228,7 +231,7 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     if st is not None:
         st.raise_if_failed()
     _call("b200moe_block_matmul", dev.index, a_ptr, a_pitch, a_scale.data_ptr(), as_m, as_kb, b_ptr, b_pitch, b_scale.data_ptr(),
-          bs_n, bs_kb, M, N, K, out.data_ptr(), dt, _pitch(out), None if st is None else st.ptr)
+          bs_n, bs_kb, M, N, K, out.data_ptr(), dt, out_pitch, None if st is None else st.ptr)
     return out
 
 
@@ -243,7 +246,7 @@ class TokenOrder:
     pair    [rows]         token * top_k + k of each row, -1 in padding and behind the last expert
     """
 
-    __slots__ = ("tokens", "top_k", "rows", "e_local", "local_expert_offset", "align", "device", "_table", "_pos_at", "_pair_at", "_ptr")
+    __slots__ = ("tokens", "top_k", "rows", "e_local", "local_expert_offset", "align", "device", "_table", "_pos_at", "_pair_at", "_pointers")
 
     def __init__(self, device, tokens, top_k, rows, e_local, local_expert_offset, align):
         self.device, self.tokens, self.top_k, self.rows = device, tokens, top_k, rows
@@ -252,7 +255,8 @@ class TokenOrder:
         self._pos_at = (2 * e_local + 4) // 4 * 4
         self._pair_at = self._pos_at + (tokens * top_k + 3) // 4 * 4
         self._table = torch.empty(self._pair_at + rows, dtype=torch.int32, device=device)
-        self._ptr = self._table.data_ptr()
+        ptr = self._table.data_ptr()
+        self._pointers = ptr + 4 * self._pos_at, ptr + 4 * self._pair_at, ptr   # addresses of pos, pair and offsets
 
     @property
     def offsets(self) -> torch.Tensor:
@@ -270,11 +274,6 @@ class TokenOrder:
     def pair(self) -> torch.Tensor:
         return self._table[self._pair_at:]
 
-    @property
-    def _pointers(self) -> Tuple[int, int, int]:
-        """Addresses of pos, pair and offsets."""
-        return self._ptr + 4 * self._pos_at, self._ptr + 4 * self._pair_at, self._ptr
-
 
 def sort_tokens(topk_ids: torch.Tensor, e_local: int = E_GLOBAL, local_expert_offset: int = 0, *, align: int = 1) -> TokenOrder:
     """Stable sort of the pairs (token, k) by expert; ids int32 or int64 [T, top_k], top_k at most 32.
@@ -288,8 +287,7 @@ def sort_tokens(topk_ids: torch.Tensor, e_local: int = E_GLOBAL, local_expert_of
     dev = topk_ids.device
     if topk_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
-    ids = _rows2d(topk_ids, "topk_ids")
-    tokens, top_k = ids.shape
+    ids, tokens, top_k, pitch = _matrix(topk_ids, "topk_ids")
     e_local, off, align = int(e_local), int(local_expert_offset), int(align)
     if not 1 <= top_k <= 32:
         raise ValueError(f"topk_ids must have 1 to 32 columns, got {top_k}")
@@ -309,30 +307,36 @@ def sort_tokens(topk_ids: torch.Tensor, e_local: int = E_GLOBAL, local_expert_of
         ws_bytes = _capi.lib().b200moe_sort_workspace_bytes(tokens, top_k, e_local)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     pos, pair, offsets = order._pointers
-    _call("b200moe_sort_tokens", dev.index, ids.data_ptr(), ids.element_size() * 8, _pitch(ids), tokens, top_k, e_local, off, align,
+    _call("b200moe_sort_tokens", dev.index, ids.data_ptr(), ids.element_size() * 8, pitch, tokens, top_k, e_local, off, align,
           offsets + 4 * (e_local + 1), offsets, pos, pair, rows, None if ws is None else ws.data_ptr(), ws_bytes)
     return order
 
 
 def _permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor]) -> torch.Tensor:
-    x = _rows2d(x, "x")
-    dev, size, H = x.device, x.element_size(), x.shape[1]
-    y = torch.empty(order.rows, H, dtype=x.dtype, device=dev) if out is None else out
-    _call("b200moe_permute_rows", dev.index, x.data_ptr(), _pitch(x) * size, H * size, size, order.tokens, order.top_k,
-          *order._pointers, order.e_local, order.rows, y.data_ptr(), _pitch(y) * size, int(out is None))
+    x, _, H, pitch = _matrix(x, "x")
+    size, y, y_pitch = x.element_size(), out, H
+    if out is None:
+        y = torch.empty(order.rows, H, dtype=x.dtype, device=x.device)
+    else:
+        y_pitch = _pitch(out)
+    _call("b200moe_permute_rows", x.device.index, x.data_ptr(), pitch * size, H * size, size, order.tokens, order.top_k,
+          *order._pointers, order.e_local, order.rows, y.data_ptr(), y_pitch * size, int(out is None))
     return y
 
 
 def _unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tensor], out: Optional[torch.Tensor]) -> torch.Tensor:
-    y = _rows2d(y, "y")
-    dev, H = y.device, y.shape[1]
+    y, _, H, pitch = _matrix(y, "y")
     w_ptr, w_pitch = None, 0
     if weights is not None:
-        weights = _rows2d(weights, "weights")
-        w_ptr, w_pitch = weights.data_ptr(), _pitch(weights)
-    res = torch.empty(order.tokens, H, dtype=y.dtype, device=dev) if out is None else out
-    _call("b200moe_unpermute_rows", dev.index, y.data_ptr(), _DTYPE[y.dtype], _pitch(y), order._pointers[0], w_ptr, w_pitch,
-          order.tokens, order.top_k, H, res.data_ptr(), _pitch(res))
+        weights, _, _, w_pitch = _matrix(weights, "weights")
+        w_ptr = weights.data_ptr()
+    res, res_pitch = out, H
+    if out is None:
+        res = torch.empty(order.tokens, H, dtype=y.dtype, device=y.device)
+    else:
+        res_pitch = _pitch(out)
+    _call("b200moe_unpermute_rows", y.device.index, y.data_ptr(), _DTYPE[y.dtype], pitch, order._pointers[0], w_ptr, w_pitch,
+          order.tokens, order.top_k, H, res.data_ptr(), res_pitch)
     return res
 
 
@@ -366,16 +370,20 @@ class _Unpermute(torch.autograd.Function):
         order, (y, weights) = ctx.order, ctx.saved_tensors
         (rows, H), dtype = ctx.y_like
         dev = dout.device
-        dout = _rows2d(dout, "grad")
+        dout, _, _, d_pitch = _matrix(dout, "grad")
         dy = torch.empty(rows, H, dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
         dw = torch.empty(order.tokens, order.top_k, dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
-        y = None if dw is None else _rows2d(y, "y")
-        w = None if weights is None else _rows2d(weights, "weights")
+        y_ptr, y_pitch, w_ptr, w_pitch = None, 0, None, 0
+        if dw is not None:
+            y, _, _, y_pitch = _matrix(y, "y")
+            y_ptr = y.data_ptr()
+        if weights is not None:
+            weights, _, _, w_pitch = _matrix(weights, "weights")
+            w_ptr = weights.data_ptr()
         pos, pair, offsets = order._pointers
-        _call("b200moe_unpermute_grad", dev.index, dout.data_ptr(), _DTYPE[dtype], _pitch(dout),
-              None if y is None else y.data_ptr(), 0 if y is None else _pitch(y), None if w is None else w.data_ptr(),
-              0 if w is None else _pitch(w), pos, pair, offsets, order.e_local, order.tokens, order.top_k, H, rows,
-              None if dy is None else dy.data_ptr(), H, None if dw is None else dw.data_ptr())
+        _call("b200moe_unpermute_grad", dev.index, dout.data_ptr(), _DTYPE[dtype], d_pitch, y_ptr, y_pitch, w_ptr, w_pitch, pos, pair,
+              offsets, order.e_local, order.tokens, order.top_k, H, rows, None if dy is None else dy.data_ptr(), H,
+              None if dw is None else dw.data_ptr())
         return dy, None, dw
 
 

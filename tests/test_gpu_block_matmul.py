@@ -140,6 +140,11 @@ def test_empty_extents_and_refusals():
         F.block_matmul(a[:, :200].contiguous(), sa, b[:, :200].contiguous(), sb, **ok)
     with pytest.raises(ValueError):
         F.block_matmul(a, sa, b.t().contiguous().t(), sb, **ok)
+    for rows in (1, 4):                                                 # elements apart, in one row and in several
+        with pytest.raises(ValueError):
+            F.block_matmul(a, sa, torch.zeros(rows, 2 * a.shape[1], dtype=torch.uint8, device=DEV)[:, ::2], sb[:1], **ok)
+    with pytest.raises(ValueError):                                     # rows that overlap in steps of a row
+        F.block_matmul(a, sa, torch.zeros(4 * a.shape[1], dtype=torch.uint8, device=DEV).as_strided((3, a.shape[1]), (a.shape[1], 2)), sb[:1], **ok)
     with pytest.raises(ValueError):
         F.block_matmul(a, sa, b, sb[:, :1], **ok)
     with pytest.raises(ValueError):
