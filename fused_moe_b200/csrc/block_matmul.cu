@@ -572,6 +572,12 @@ constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + kScaleRing * 2 * 
 constexpr int kPairLaunchRegs = 168, kPairCtrlRegs = 72, kPairPromoRegs = 216;
 static_assert(128 * (kPairLaunchRegs - kPairCtrlRegs) >= 256 * (kPairPromoRegs - kPairLaunchRegs),
               "setmaxnreg.inc would wait for registers that nobody releases");
+// A CTA that asks for tensor memory waits until there is enough, and CTAs of a cluster wait for one another: so no two of these
+// CTAs may be on an SM whose accumulators do not fit together.  Shared memory sees to it.
+constexpr int kSmSmemBytes = 228 * 1024;
+static_assert(3 * mid_smem_bytes(2) > kSmSmemBytes, "three CTAs with 256 columns each");
+static_assert(mid_smem_bytes(4) + mid_smem_bytes(2) > kSmSmemBytes && kPairSmemBytes + mid_smem_bytes(2) > kSmSmemBytes,
+              "a CTA with all 512 columns beside another");
 constexpr int kPairSuper = 8;                    // M tiles that run beside each other on the same N tiles
 
 __device__ __forceinline__ void pair_tmem_alloc(uint32_t smem_result_addr, uint32_t ncols) {
