@@ -25,7 +25,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 
-HOST_FILES = ("__init__.py", "_capi.py", "build.py", "kernel.py")
+# what the package imports when it is imported, and the build
+HOST_FILES = ("__init__.py", "_capi.py", "build.py", "kernel.py", "ops.py")
 
 
 def collect_sources():
