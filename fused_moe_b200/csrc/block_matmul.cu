@@ -332,9 +332,11 @@ __device__ __forceinline__ bool count_poll(uint32_t addr, uint32_t target, volat
   }
 }
 
-__device__ __forceinline__ void report_status(const MatmulParams& p, const int* abort, const int* status) {
-  if (abort[0] && p.status) {
+// (The code goes last: who finds it finds the detail too.  A wait for copies or MMAs in flight that gave up counts like any other.)
+__device__ __forceinline__ void report_status(const MatmulParams& p, const int* status) {
+  if (status[kStatusCode] && p.status) {
     p.status[1] = status[kStatusDetail];
+    __threadfence_system();
     p.status[0] = status[kStatusCode];
     __threadfence_system();
   }
@@ -409,7 +411,7 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
   __shared__ uint64_t s_bars[2 * kStages + ACC + 2 + 2 * kScaleRing];
   __shared__ uint32_t s_read[ACC];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort[2], s_status[2];
+  __shared__ int s_abort[3], s_status[2];   // waits of the loops, for copies in flight, for MMAs in flight: each gives up for itself
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bar_full = smem_u32(s_bars), bar_empty = bar_full + 8 * kStages;
   const uint32_t bar_done = bar_empty + 8 * kStages, bar_drain = bar_done + 8 * ACC, count_read = smem_u32(s_read);
@@ -432,7 +434,7 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
     }
     mbar_init(bar_drain, 1);
     mbar_init(bar_drain + 8, 1);
-    s_abort[0] = s_abort[1] = 0;
+    s_abort[0] = s_abort[1] = s_abort[2] = 0;
     s_status[0] = s_status[1] = 0;
     fence_mbar_init();
     tma_prefetch_desc(&p.tmap_a);
@@ -491,7 +493,7 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
         __syncwarp();
       }
       if (elect_one()) tc_commit(bar_drain + 8 * me);   // all MMAs must have read the ring and written tensor memory before either is released
-      (void)mbar_poll(bar_drain + 8 * me, 0, abort_flag + 1, s_status, 5);
+      (void)mbar_poll(bar_drain + 8 * me, 0, abort_flag + 2, s_status, 5);
     } else if (warp == 3) {
       make_factors<1, 4>(
           p, factors, 0, m0, n0 / kBlockK, kb0, kb1, lane,
@@ -553,7 +555,7 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, ACC * kTile);
-  if (threadIdx.x == 0) report_status(p, s_abort, s_status);
+  if (threadIdx.x == 0) report_status(p, s_status);
 }
 
 // ------------------------------ 256 x 256 tiles of a CTA pair ------------------------------
@@ -642,7 +644,7 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
   __shared__ uint64_t s_bars[2 * S + 4 + 2 + 2 * kScaleRing];
   __shared__ uint32_t s_read[4];                           // leader's: [half][2] warps of both CTAs that have read an accumulator
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort[2], s_status[2];
+  __shared__ int s_abort[3], s_status[2];   // waits of the loops, for copies in flight, for MMAs in flight: each gives up for itself
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bar_full = smem_u32(s_bars);              // leader's: a stage of both CTAs has landed
   const uint32_t bar_empty = bar_full + 8 * S;             // both: the MMAs have read a stage
@@ -670,7 +672,7 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
       mbar_init(bar_factors + 8 * r, 1);
       mbar_init(bar_slot + 8 * r, 8);
     }
-    s_abort[0] = s_abort[1] = 0;
+    s_abort[0] = s_abort[1] = s_abort[2] = 0;
     s_status[0] = s_status[1] = 0;
     fence_mbar_init();
     tma_prefetch_desc(&p.tmap_a);
@@ -715,6 +717,9 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
         if (rank == 0) (void)mbar_poll(bar_full + 8 * (j % S), (j / S) & 1, abort_flag + 1, s_status, 12);
         (void)mbar_poll(bar_empty + 8 * (j % S), (j / S) & 1, abort_flag + 1, s_status, 12);
       }
+      // The issuers are the leader's: only here, behind the last K block, is the wait for their MMAs one of a hand-off's length.
+      if (rank != 0)
+        for (int i = 0; i < 2; ++i) (void)mbar_poll(bar_drain + 8 * i, 0, abort_flag + 2, s_status, 15);
     } else if (warp == 1 || warp == 2) {
       // (The loop's form: see the other kernel.  What makes the two looks at a stage's barrier safe: this warp's last turn waited
       // until K block it - 4 had been read back, so it - 5, the stage's use before, has landed; and behind the first count_poll
@@ -744,8 +749,10 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
         if (!__all_sync(0xffffffffu, ok)) break;
         seen = __all_sync(0xffffffffu, seen);
       }
-      if (rank == 0 && elect_one()) pair_commit(bar_drain + 8 * me);
-      (void)mbar_poll(bar_drain + 8 * me, 0, abort_flag + 1, s_status, 15);
+      if (rank == 0) {
+        if (elect_one()) pair_commit(bar_drain + 8 * me);
+        (void)mbar_poll(bar_drain + 8 * me, 0, abort_flag + 2, s_status, 15);
+      }
     } else if (warp == 3) {
       uint32_t it = 0;
       for (int tile = first; tile < tiles; tile += stride, it += kblocks) {
@@ -805,7 +812,7 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
   cluster_wait();
   tc_fence_after();
   if (warp == 1) pair_tmem_dealloc(tmem, 512);
-  if (threadIdx.x == 0) report_status(p, s_abort, s_status);
+  if (threadIdx.x == 0) report_status(p, s_status);
 }
 
 // Whether every CTA of 128 x 128 tiles with S parts of K has an SM alone.  A cluster's CTAs have to be neighbours, for which not
