@@ -26,6 +26,8 @@ constexpr int kTile = 128;
 constexpr int kOperandBytes = kTile * kBlockK;   // 16 KiB
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kMaxSplit = 8;
+// What a row becomes whose sum a bounded wait cut short: nothing that could pass for a result.
+constexpr float kGivenUp = __builtin_nanf("");
 
 struct MatmulParams {
   CUtensorMap tmap_a, tmap_b;
@@ -45,6 +47,9 @@ struct MatmulParams {
 
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, float a, float b, float c, float d) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+__device__ __forceinline__ void st_cluster_s32(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ float4 ld_shared_v4(uint32_t addr) {
   float4 v;
@@ -90,6 +95,12 @@ __device__ __forceinline__ void store4(const MatmulParams& p, int m, int n, floa
     if (n + 2 < p.N) dst[2] = (uint16_t)hi;
     if (n + 3 < p.N) dst[3] = (uint16_t)(hi >> 16);
   }
+}
+
+// Columns [n, n + 128) of row m for a row given up.
+__device__ __forceinline__ void store_given_up(const MatmulParams& p, int m, int n) {
+#pragma unroll 1
+  for (int i = 0; i < kTile; i += 4) store4(p, m, n + i, make_float4(kGivenUp, kGivenUp, kGivenUp, kGivenUp));
 }
 
 // A row's word i (of 64 or 128), zero behind the last.
@@ -335,7 +346,7 @@ __device__ __forceinline__ bool count_poll(uint32_t addr, uint32_t target, volat
 // (The code goes last: who finds it finds the detail too.  A wait for copies or MMAs in flight that gave up counts like any other.)
 __device__ __forceinline__ void report_status(const MatmulParams& p, const int* status) {
   if (status[kStatusCode] && p.status) {
-    p.status[1] = status[kStatusDetail];
+    if (status[kStatusDetail]) p.status[1] = status[kStatusDetail];   // (0: it was another CTA of the cluster that gave up)
     __threadfence_system();
     p.status[0] = status[kStatusCode];
     __threadfence_system();
@@ -504,6 +515,9 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
     if (split > 1) {         // the promotion warps' two barriers, see there
       cluster_arrive();
       cluster_wait();
+      if (warp == 3 && lane < split && *abort_flag)   // a part of the sum is lost: the cluster's other CTAs learn of it
+        st_cluster_s32(map_to_rank(smem_u32(s_status + kStatusCode), (uint32_t)lane), (int)B200MOE_ERR_DEVICE_TIMEOUT);
+      __syncwarp();
       cluster_arrive();
       cluster_wait();
     }
@@ -555,7 +569,10 @@ block_matmul_kernel(const __grid_constant__ MatmulParams p) {
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, ACC * kTile);
-  if (threadIdx.x == 0) report_status(p, s_status);
+  if (__builtin_expect(s_status[kStatusCode], 0)) {
+    store_given_up(p, m0 + (threadIdx.x & 127), n0);   // (over what was stored: a choice before took 2 to 7 % of a small call, this 0 to 2)
+    if (threadIdx.x == 0) report_status(p, s_status);
+  }
 }
 
 // ------------------------------ 256 x 256 tiles of a CTA pair ------------------------------
@@ -773,7 +790,8 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
     const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + half * 2 * kTile;
     uint32_t it = 0, seen_f = 0, seen_d = 0;   // seen: the coming K block's factors, accumulator are known to be there (looked at below)
     bool alive = true;
-    for (int tile = first; tile < tiles && alive; tile += stride) {
+    int tile = first;
+    for (; tile < tiles; tile += stride) {
       int m0, n0;
       pair_tile(p, tile, &m0, &n0);
       m0 += rank * kTile + q * 32;
@@ -804,6 +822,13 @@ block_matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
       }
       if (!alive) break;
       store_row128(p, m0 + lane, n0, acc);
+    }
+    for (; tile < tiles; tile += stride) {   // (given up: this tile and those to come)
+      int m0, n0;
+      pair_tile(p, tile, &m0, &n0);
+      m0 += rank * kTile + q * 32 + lane;
+      n0 += half * kTile;
+      store_given_up(p, m0, n0);
     }
   }
   tc_fence_before();

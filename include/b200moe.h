@@ -291,6 +291,7 @@ B200MOE_API int b200moe_quantize(const void* x, int dtype, int64_t row_stride, i
  *  out      [M, N] of `out_dtype` (fp32, bf16, fp16), `out_row_stride` elements
  *  status   optional device-accessible int32[2] (e.g. host-mapped), written only when a bounded device-side wait gave up:
  *           [0] = B200MOE_ERR_DEVICE_TIMEOUT, [1] = where.
+ *           What such a wait cuts short is stored as NaN, with or without `status`.
  * K a multiple of 16 (the last block may be short); M, N any. */
 B200MOE_API int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride,
                          const float* a_scale, int64_t a_scale_stride_m, int64_t a_scale_stride_kb,
