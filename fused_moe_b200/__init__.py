@@ -7,7 +7,7 @@
 loaded on first use and its absence is an error, never a fallback.
 """
 from .kernel import run, custom_kernel, route, MoEError  # noqa: F401
-from .ops import TokenOrder, block_matmul, permute, quantize, sort_tokens, unpermute  # noqa: F401
+from .ops import TokenOrder, block_matmul, check_status, permute, quantize, sort_tokens, unpermute  # noqa: F401
 
 __all__ = ["run", "custom_kernel", "route", "MoEError", "quantize", "block_matmul", "sort_tokens", "permute", "unpermute",
-           "TokenOrder"]
+           "TokenOrder", "check_status"]

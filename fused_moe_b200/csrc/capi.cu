@@ -43,6 +43,7 @@ thread_local int* g_status_mirror = nullptr;
 std::mutex g_mutex;
 EncodeTiledFn g_encode = nullptr;
 DeviceInfo g_dev[64];
+int* g_status_words[64];      // per device, pinned; kept until the process ends
 
 }  // namespace
 
@@ -614,6 +615,28 @@ int b200moe_selftest_wait_timeout(void* status_int4, void* stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   CUDA_TRY(cudaMemsetAsync(status_int4, 0, 16, st));
   CUDA_TRY(launch_wait_timeout_selftest(reinterpret_cast<int*>(status_int4), st));
+  return B200MOE_OK;
+}
+
+int b200moe_status_words(int32_t** words) {
+  if (!words) return B200MOE_ERR_INVALID_ARGUMENT;
+  *words = nullptr;
+  int dev = 0;
+  CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return B200MOE_ERR_INVALID_ARGUMENT;
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (!g_status_words[dev]) {
+    // an allocation of the host's, no part of what a stream may be capturing meanwhile
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+    void* host = nullptr;
+    const cudaError_t e = cudaHostAlloc(&host, 4 * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+    CUDA_TRY(e);
+    memset(host, 0, 4 * sizeof(int));
+    g_status_words[dev] = reinterpret_cast<int*>(host);
+  }
+  *words = g_status_words[dev];
   return B200MOE_OK;
 }
 

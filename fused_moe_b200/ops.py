@@ -14,7 +14,9 @@ The layer from parts is the sequence route, sort_tokens, permute, quantize, bloc
 block_matmul, unpermute.  All results repeat bit for bit (there are no atomics on values), every call is asynchronous on the
 current stream of its tensors' device, can be captured into a CUDA graph and allocates only its results (and the sort, above
 16384 pairs, a scratch tensor) from torch's allocator.  Errors: ``TypeError`` / ``ValueError`` for arguments, ``RuntimeError``
-for tensors that are not on one CUDA device, ``MoEError`` for what the library refuses.  A backward pass is captured like any of
+for tensors that are not on one CUDA device, ``MoEError`` for what the library refuses, and at the next call of any operator on the
+device after a ``block_matmul`` there gave up on a bounded wait (its result holds NaN then).  A replayed graph makes no call:
+``check_status`` looks.  A backward pass is captured like any of
 torch's: after a warm-up on a side stream, with no earlier graph of the same leaves alive (torch warns about its AccumulateGrad
 node and the capture fails).  Gradients are first order.
 
@@ -45,8 +47,45 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _functions: Dict[str, object] = {}
 
 
+class _Status:
+    """Pinned words of one device where a kernel that gave up on a bounded wait leaves its code."""
+
+    def __init__(self, index: int):
+        words = C.c_void_p()
+        with torch.cuda.device(index):
+            _capi.check(_capi.lib().b200moe_status_words(C.byref(words)), "b200moe_status_words")
+        self.ptr = words.value
+        self.view = (C.c_int32 * 4).from_address(self.ptr)
+
+    def raise_if_failed(self) -> None:
+        if self.view[0]:
+            code, where = self.view[0], self.view[1]
+            self.view[0] = 0
+            raise MoEError(code, "device status of an earlier b200moe_block_matmul on this device", f"detail={where}")
+
+
+_status: Dict[int, _Status] = {}
+
+
+def check_status(device=None) -> None:
+    """Waits for the device (None: the current one) and raises ``MoEError`` if a ``block_matmul`` on it gave up on a bounded wait
+    since the last look, in a replayed graph too.  Such a product holds NaN where a sum was cut short."""
+    dev = torch.device("cuda" if device is None else device)
+    if dev.type != "cuda":
+        raise RuntimeError(f"device is {dev}: fused_moe_b200 runs on CUDA devices only (there is no CPU path)")
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    torch.cuda.synchronize(index)
+    st = _status.get(index)
+    if st is not None:
+        st.raise_if_failed()
+
+
 def _call(name: str, index: int, *args) -> None:
-    """Library call with its device current, on that device's current stream (the last argument)."""
+    """Library call with its device current, on that device's current stream (the last argument).  What an earlier call there left
+    in the status words is raised first."""
+    st = _status.get(index)
+    if st is not None:
+        st.raise_if_failed()
     fn = _functions.get(name)
     if fn is None:
         fn = _functions[name] = getattr(_capi.lib(), name)
@@ -142,24 +181,6 @@ def quantize(x: torch.Tensor, *, swiglu: bool = False, scale_layout: str = "kt")
 
 # ---- block-scaled product ----
 
-class _Status:
-    """Pinned words of one device where a kernel that gave up on a bounded wait leaves its code."""
-
-    def __init__(self):
-        self.words = torch.zeros(4, dtype=torch.int32).pin_memory()
-        self.ptr = self.words.data_ptr()
-        self.view = (C.c_int32 * 4).from_address(self.ptr)
-
-    def raise_if_failed(self):
-        if self.view[0]:
-            code, where = self.view[0], self.view[1]
-            self.view[0] = 0
-            raise MoEError(code, "device status of an earlier b200moe_block_matmul on this device", f"detail={where}")
-
-
-_status: Dict[int, _Status] = {}
-
-
 def _block_scale_strides(scale: torch.Tensor, rows: int, blocks: int, layout: str, what: str) -> Tuple[int, int]:
     """(stride over rows, stride over K blocks) of a scale tensor, in elements."""
     if scale.dtype != torch.float32:
@@ -226,12 +247,10 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     if M == 0 or N == 0:
         return out
     st = _status.get(dev.index)
-    if st is None and not torch.cuda.is_current_stream_capturing():   # (pinned memory cannot be had during a capture)
-        st = _status.setdefault(dev.index, _Status())
-    if st is not None:
-        st.raise_if_failed()
+    if st is None:
+        st = _status.setdefault(dev.index, _Status(dev.index))
     _call("b200moe_block_matmul", dev.index, a_ptr, a_pitch, a_scale.data_ptr(), as_m, as_kb, b_ptr, b_pitch, b_scale.data_ptr(),
-          bs_n, bs_kb, M, N, K, out.data_ptr(), dt, out_pitch, None if st is None else st.ptr)
+          bs_n, bs_kb, M, N, K, out.data_ptr(), dt, out_pitch, st.ptr)
     return out
 
 

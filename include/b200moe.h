@@ -284,6 +284,11 @@ B200MOE_API int b200moe_quantize(const void* x, int dtype, int64_t row_stride, i
                      uint8_t* codes, int64_t codes_row_stride,
                      float* scale, int64_t scale_stride_t, int64_t scale_stride_kb, void* stream);
 
+/* Four words of pinned, device-accessible host memory of the current device, zeroed once and the library's until the process
+ * ends, the same at every call: what a caller can give b200moe_block_matmul as `status`.  Allowed while a stream is captured, so
+ * that a graph whose first call is a captured one can report too. */
+B200MOE_API int b200moe_status_words(int32_t** words);
+
 /* out[m,n] = sum_b a_scale[m,b] * b_scale[n/128,b] * sum_{k in block b} a[m,k] * b[n,k], accumulated in fp32, rounded once.
  *  a        e4m3 [M, K], b e4m3 [N, K] (the experts' weight layout); row strides in bytes, multiples of 16; bases 16-byte aligned
  *  a_scale  fp32, element (m, b) at a_scale[m*a_scale_stride_m + b*a_scale_stride_kb]
