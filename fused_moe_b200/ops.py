@@ -18,7 +18,7 @@ for tensors that are not on one CUDA device, ``MoEError`` for what the library r
 device after a ``block_matmul`` there gave up on a bounded wait (its result holds NaN then).  A replayed graph makes no call:
 ``check_status`` looks.  A backward pass is captured like any of
 torch's: after a warm-up on a side stream, with no earlier graph of the same leaves alive (torch warns about its AccumulateGrad
-node and the capture fails).  Gradients are first order.
+node and the capture fails).  Gradients are first order and reverse mode: tensors with a forward-mode tangent are refused.
 
 The reference has no counterparts: its only public function is the fused layer (solution/python/kernel.py:642-648).
 """
@@ -28,6 +28,7 @@ import ctypes as C
 from typing import Dict, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 from ._capi import MoEError
@@ -112,6 +113,14 @@ def _no_gradient(what: str) -> RuntimeError:
     return RuntimeError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
+def _refuse_duals(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raises for a tensor with a forward-mode tangent, which a library call would drop without a word (it does not make
+    ``requires_grad`` true).  Called only where a level of dual numbers is open."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative: detach its inputs")
+
+
 def _matrix(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
     """(``t``, rows, columns, row stride in elements) with unit inner stride and rows that do not overlap (a copy where ``t`` has not);
     extents that 32 bits hold.  The stride of a single row is free: torch may say anything."""
@@ -162,6 +171,8 @@ def quantize(x: torch.Tensor, *, swiglu: bool = False, scale_layout: str = "kt")
         raise ValueError(f"scale_layout must be 'kt' or 'tk', got {scale_layout!r}")
     if x.requires_grad and torch.is_grad_enabled():
         raise _no_gradient("quantize")
+    if forward_ad._current_level >= 0:
+        _refuse_duals("quantize", x)
     x, rows, cols, pitch = _matrix(x, "x")
     if swiglu:
         if cols % 2:
@@ -211,6 +222,8 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
         raise _other_device(dev, a_scale=a_scale, b=b, b_scale=b_scale)
     if (a_scale.requires_grad or b_scale.requires_grad or a.requires_grad or b.requires_grad) and torch.is_grad_enabled():
         raise _no_gradient("block_matmul")
+    if forward_ad._current_level >= 0:
+        _refuse_duals("block_matmul", a, a_scale, b, b_scale, out)
     if a.dtype not in _CODES or b.dtype not in _CODES:
         raise TypeError(f"a and b must be float8_e4m3fn (or its uint8 bit pattern), got {a.dtype} and {b.dtype}")
     a, M, K, a_pitch = _matrix(a, "a")
@@ -367,9 +380,15 @@ def _unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tenso
 
 
 def _first_order(backward):
-    """``once_differentiable`` where a graph of the gradient is asked for; elsewhere without what that wrapper takes (4 us)."""
+    """``once_differentiable`` where a graph of the gradient is asked for; elsewhere without what that wrapper takes (4 us).  A
+    gradient that is a dual number is refused like an argument."""
     guarded = torch.autograd.function.once_differentiable(backward)
-    return staticmethod(lambda ctx, grad: guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad))
+
+    def run(ctx, grad):
+        if forward_ad._current_level >= 0:
+            _refuse_duals("the gradient", grad)
+        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+    return staticmethod(run)
 
 
 class _Permute(torch.autograd.Function):
@@ -429,6 +448,8 @@ def permute(x: torch.Tensor, order: TokenOrder, *, out: Optional[torch.Tensor] =
         raise ValueError(f"x must be [{order.tokens}, H], got {tuple(x.shape)}")
     if x.element_size() not in (1, 2, 4) or x.is_complex():
         raise TypeError(f"x must have elements of 1, 2 or 4 bytes, got {x.dtype}")
+    if forward_ad._current_level >= 0:
+        _refuse_duals("permute", x, out)
     if x.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise RuntimeError("permute with out= has no gradient: detach x or leave out away")
@@ -462,6 +483,8 @@ def unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tensor
             raise TypeError(f"weights must be float32, got {weights.dtype}")
         if tuple(weights.shape) != (order.tokens, order.top_k):
             raise ValueError(f"weights must be [{order.tokens}, {order.top_k}], got {tuple(weights.shape)}")
+    if forward_ad._current_level >= 0:
+        _refuse_duals("unpermute", y, weights, out)
     if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
         if out is not None:
             raise RuntimeError("unpermute with out= has no gradient: detach its inputs or leave out away")
