@@ -122,13 +122,15 @@ def _refuse_duals(what: str, *tensors: Optional[torch.Tensor]) -> None:
 
 
 def _matrix(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
-    """(``t``, rows, columns, row stride in elements) with unit inner stride and rows that do not overlap (a copy where ``t`` has not);
-    extents that 32 bits hold.  The stride of a single row is free: torch may say anything."""
+    """(``t``, rows, columns, row stride in elements) with unit inner stride, rows that do not overlap and values as they are stored (a
+    copy where ``t`` has not: ``z.conj().imag`` is stored with the other sign); extents that 32 bits hold.  The stride of a single row is free: torch may say anything."""
     if t.dim() != 2:
         raise ValueError(f"{what} must be 2-D, got shape {tuple(t.shape)}")
     rows, cols = t.shape
     if rows > _INT_MAX or cols > _INT_MAX:
         raise ValueError(f"{what} must have at most {_INT_MAX} rows and columns, got shape {tuple(t.shape)}")
+    if t.is_neg():
+        t = t.resolve_neg()
     if t.is_contiguous():
         return t, rows, cols, cols
     s0, s1 = t.stride()
@@ -147,6 +149,8 @@ def _check_out(out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, de
         raise ValueError(f"out must be {dtype} {list(shape)} on {dev}, got {out.dtype} {list(out.shape)} on {out.device}")
     if (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1]):
         raise ValueError("out must have unit inner stride and rows that do not overlap")
+    if out.is_neg():
+        raise ValueError("out must not be the imaginary part of a conjugate, which is stored with the other sign")
     if out.requires_grad:
         raise RuntimeError("out must not require a gradient")
 
@@ -237,6 +241,8 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     if scale_layout not in ("kt", "tk"):
         raise ValueError(f"scale_layout must be 'kt' or 'tk', got {scale_layout!r}")
     blocks = -(-K // BLOCK)
+    if a_scale.is_neg() or b_scale.is_neg():
+        a_scale, b_scale = a_scale.resolve_neg(), b_scale.resolve_neg()
     as_m, as_kb = _block_scale_strides(a_scale, M, blocks, scale_layout, "a_scale")
     bs_n, bs_kb = _block_scale_strides(b_scale, -(-N // BLOCK), blocks, "tk", "b_scale")
     a_ptr, b_ptr = a.data_ptr(), b.data_ptr()
