@@ -155,6 +155,11 @@ def _check_out(out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, de
         raise RuntimeError("out must not require a gradient")
 
 
+def _written(out: torch.Tensor) -> None:
+    """Tells autograd that ``out`` changed, as torch's own functions do: a graph that saved it refuses to go backward through it."""
+    torch.autograd.graph.increment_version(out)
+
+
 # ---- quantisation ----
 
 def quantize(x: torch.Tensor, *, swiglu: bool = False, scale_layout: str = "kt") -> Tuple[torch.Tensor, torch.Tensor]:
@@ -263,6 +268,7 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
             raise TypeError(f"out must be float32, bfloat16 or float16, got {out.dtype}")
         _check_out(out, (M, N), out.dtype, dev)
         out_pitch = _pitch(out)
+        _written(out)
     if M == 0 or N == 0:
         return out
     st = _status.get(dev.index)
@@ -366,6 +372,8 @@ def _permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor]) ->
         y_pitch = _pitch(out)
     _call("b200moe_permute_rows", x.device.index, x.data_ptr(), pitch * size, H * size, size, order.tokens, order.top_k,
           *order._pointers(), order.e_local, order.rows, y.data_ptr(), y_pitch * size, int(out is None))
+    if out is not None:
+        _written(out)
     return y
 
 
@@ -382,6 +390,8 @@ def _unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tenso
         res_pitch = _pitch(out)
     _call("b200moe_unpermute_rows", y.device.index, y.data_ptr(), _DTYPE[y.dtype], pitch, order._pointers()[0], w_ptr, w_pitch,
           order.tokens, order.top_k, H, res.data_ptr(), res_pitch)
+    if out is not None:
+        _written(out)
     return res
 
 
