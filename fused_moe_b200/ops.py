@@ -40,9 +40,10 @@ _CODES = (torch.float8_e4m3fn, torch.uint8)
 _DTYPE = {torch.float32: _capi.F32, torch.bfloat16: _capi.BF16, torch.float16: _capi.F16}
 
 
-# what a call asks of torch besides its tensors, without the Python layers above: half a microsecond instead of four
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# what a call asks of torch besides its tensors, without the Python layers above: half a microsecond instead of four (None where
+# torch was built without CUDA, and with it any tensor that a call would take)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 _functions: Dict[str, object] = {}
