@@ -66,6 +66,7 @@ SIGNATURES = {
     "b200moe_ep_combine_peers": (_I, [_P, _P, _P, _I, _I, _I, _P, _P]),
     "b200moe_quantize": (_I, [_P, _I, _L, _I, _I, _I, _P, _L, _P, _L, _L, _P]),
     "b200moe_status_words": (_I, [C.POINTER(_P)]),
+    "b200moe_block_matmul_form": (_I, [_I, _I, _I, _L, _L, _I]),
     "b200moe_block_matmul": (_I, [_P, _L, _P, _L, _L, _P, _L, _P, _L, _L, _I, _I, _I, _P, _I, _L, _P, _P]),
     "b200moe_sort_rows": (_L, [_L, _I, _I, _I]),
     "b200moe_sort_workspace_bytes": (_L, [_L, _I, _I]),

@@ -868,6 +868,34 @@ long long pair_cost(long long tiles, int kblocks, int num_sms) {
   return (tiles + pairs - 1) / pairs * (kblocks * 530ll + 1500);
 }
 
+// How a product is made: 256 x 256 tiles of CTA pairs, or 128 x 128 tiles with `split` parts of K, each CTA alone on its SM or not.
+struct MatmulForm {
+  bool pair;
+  int split;
+  bool alone;
+};
+MatmulForm matmul_form(int M, long long m_tiles, long long n_tiles, int kblocks, bool rough, int num_sms) {
+  const int rows = M < kTile ? M : kTile;
+  MatmulForm f = {false, 1, false};
+  long long cost = mid_cost(m_tiles * n_tiles, kblocks, rows, 1, rough, num_sms);
+  for (int S : {2, 3, 4, 8}) {
+    if (2 * S > kblocks) break;
+    const long long c = mid_cost(m_tiles * n_tiles, kblocks, rows, S, rough, num_sms);
+    if (c < cost) {
+      cost = c;
+      f.split = S;
+    }
+  }
+  if (pair_cost(((m_tiles + 1) / 2) * ((n_tiles + 1) / 2), kblocks, num_sms) < cost) return {true, 1, true};
+  f.alone = mid_alone(m_tiles * n_tiles * f.split, f.split, num_sms);
+  return f;
+}
+// Rows that do not start on sectors (32 bytes).
+bool rough_rows(int64_t a_row_stride, int64_t b_row_stride) { return (a_row_stride | b_row_stride) % 32 != 0; }
+bool too_many_tiles(int M, int N, long long m_tiles, long long n_tiles) {
+  return m_tiles * n_tiles * kMaxSplit > 0x7fffffffll || M > 0x7fffff00 || N > 0x7fffff00;
+}
+
 }  // namespace
 
 cudaError_t configure_block_matmul() {
@@ -881,6 +909,14 @@ cudaError_t configure_block_matmul() {
 }  // namespace b200moe
 
 using namespace b200moe;
+
+extern "C" int b200moe_block_matmul_form(int M, int N, int K, int64_t a_row_stride, int64_t b_row_stride, int num_sms) {
+  if (M < 1 || N < 1 || K < 1 || num_sms < 1 || a_row_stride < K || b_row_stride < K) return B200MOE_ERR_INVALID_ARGUMENT;
+  const long long m_tiles = ((long long)M + kTile - 1) / kTile, n_tiles = ((long long)N + kTile - 1) / kTile;
+  if (K % 16 != 0 || too_many_tiles(M, N, m_tiles, n_tiles)) return B200MOE_ERR_UNSUPPORTED_SHAPE;
+  const MatmulForm f = matmul_form(M, m_tiles, n_tiles, (K + kBlockK - 1) / kBlockK, rough_rows(a_row_stride, b_row_stride), num_sms);
+  return f.pair ? 0 : f.alone ? f.split : 16 + f.split;
+}
 
 extern "C" int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride, const float* a_scale, int64_t a_scale_stride_m,
                                     int64_t a_scale_stride_kb, const uint8_t* b, int64_t b_row_stride, const float* b_scale,
@@ -897,7 +933,7 @@ extern "C" int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride, cons
       reinterpret_cast<uintptr_t>(out) % size != 0)
     return B200MOE_ERR_MISALIGNED;
   const long long m_tiles = ((long long)M + kTile - 1) / kTile, n_tiles = ((long long)N + kTile - 1) / kTile;
-  if (m_tiles * n_tiles * kMaxSplit > 0x7fffffffll || M > 0x7fffff00 || N > 0x7fffff00) return B200MOE_ERR_UNSUPPORTED_SHAPE;
+  if (too_many_tiles(M, N, m_tiles, n_tiles)) return B200MOE_ERR_UNSUPPORTED_SHAPE;
   int num_sms = 0;
   int rc = ensure_device(&num_sms);
   if (rc != B200MOE_OK) return rc;
@@ -919,39 +955,26 @@ extern "C" int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride, cons
   p.status = status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 
-  const int rows = M < kTile ? M : kTile;
-  const bool rough = (a_row_stride | b_row_stride) % 32 != 0;
-  p.split = 1;
-  long long cost = mid_cost(m_tiles * n_tiles, p.kblocks, rows, 1, rough, num_sms);
-  for (int S : {2, 3, 4, 8}) {
-    if (2 * S > p.kblocks) break;
-    const long long c = mid_cost(m_tiles * n_tiles, p.kblocks, rows, S, rough, num_sms);
-    if (c < cost) {
-      cost = c;
-      p.split = S;
-    }
-  }
-  const long long pair_tiles = ((m_tiles + 1) / 2) * ((n_tiles + 1) / 2);
-  if (pair_cost(pair_tiles, p.kblocks, num_sms) < cost) {
-    p.split = 1;
+  const MatmulForm form = matmul_form(M, m_tiles, n_tiles, p.kblocks, rough_rows(a_row_stride, b_row_stride), num_sms);
+  p.split = form.split;
+  if (form.pair) {
     if ((rc = make_tmap(&p.tmap_a, a, (uint64_t)M, (uint64_t)K, (uint64_t)a_row_stride, kTile)) != B200MOE_OK) return rc;
     if ((rc = make_tmap(&p.tmap_b, b, (uint64_t)N, (uint64_t)K, (uint64_t)b_row_stride, kTile / 2)) != B200MOE_OK) return rc;
     p.m_tiles = (int)((m_tiles + 1) / 2);
     p.n_tiles = (int)((n_tiles + 1) / 2);
-    const long long pairs = num_sms / 2;
+    const long long pairs = num_sms / 2, pair_tiles = (long long)p.m_tiles * p.n_tiles;
     CUDA_TRY(launch_chained_cluster(block_matmul_pair_kernel, dim3((unsigned)(2 * (pair_tiles < pairs ? pair_tiles : pairs))), dim3(kPairThreads),
                                     kPairSmemBytes, st, 2, p));
     return B200MOE_OK;
   }
   if ((rc = make_tmap(&p.tmap_b, b, (uint64_t)N, (uint64_t)K, (uint64_t)b_row_stride, kTile)) != B200MOE_OK) return rc;
   // fewer rows than a tile has are a smaller copy
-  p.box_rows = rows;
+  p.box_rows = M < kTile ? M : kTile;
   if ((rc = make_tmap(&p.tmap_a, a, (uint64_t)M, (uint64_t)K, (uint64_t)a_row_stride, (uint32_t)p.box_rows)) != B200MOE_OK) return rc;
   p.m_tiles = (int)m_tiles;
   p.n_tiles = (int)n_tiles;
-  const long long ctas = m_tiles * n_tiles * p.split;
-  const bool alone = mid_alone(ctas, p.split, num_sms);
-  CUDA_TRY(launch_chained_cluster(alone ? block_matmul_kernel<4> : block_matmul_kernel<2>, dim3((unsigned)ctas), dim3(kMidThreads),
-                                  mid_smem_bytes(alone ? 4 : 2), st, p.split, p));
+  CUDA_TRY(launch_chained_cluster(form.alone ? block_matmul_kernel<4> : block_matmul_kernel<2>,
+                                  dim3((unsigned)(m_tiles * n_tiles * p.split)), dim3(kMidThreads), mid_smem_bytes(form.alone ? 4 : 2), st,
+                                  p.split, p));
   return B200MOE_OK;
 }

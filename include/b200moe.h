@@ -289,6 +289,11 @@ B200MOE_API int b200moe_quantize(const void* x, int dtype, int64_t row_stride, i
  * that a graph whose first call is a captured one can report too. */
 B200MOE_API int b200moe_status_words(int32_t** words);
 
+/* Which kernel b200moe_block_matmul takes for such sizes and row strides on a GPU of num_sms SMs (no CUDA call is made): 0 for 256 x 256
+ * tiles of CTA pairs; S = 1, 2, 3, 4 or 8 for 128 x 128 tiles with K divided over S CTAs, each alone on its SM; 16 + S where two
+ * share an SM.  The order of the sums goes with S.  Negative: a status. */
+B200MOE_API int b200moe_block_matmul_form(int M, int N, int K, int64_t a_row_stride, int64_t b_row_stride, int num_sms);
+
 /* out[m,n] = sum_b a_scale[m,b] * b_scale[n/128,b] * sum_{k in block b} a[m,k] * b[n,k], accumulated in fp32, rounded once.
  *  a        e4m3 [M, K], b e4m3 [N, K] (the experts' weight layout); row strides in bytes, multiples of 16; bases 16-byte aligned
  *  a_scale  fp32, element (m, b) at a_scale[m*a_scale_stride_m + b*a_scale_stride_kb]
