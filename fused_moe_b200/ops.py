@@ -86,7 +86,7 @@ def _call(name: str, index: int, *args) -> None:
     """Library call with its device current, on that device's current stream (the last argument).  What an earlier call there left
     in the status words is raised first."""
     st = _status.get(index)
-    if st is not None:
+    if st is not None and st.view[0]:
         st.raise_if_failed()
     fn = _functions.get(name)
     if fn is None:
@@ -291,7 +291,7 @@ class TokenOrder:
     pair    [rows]         token * top_k + k of each row, -1 in padding and behind the last expert
     """
 
-    __slots__ = ("tokens", "top_k", "rows", "e_local", "local_expert_offset", "align", "_table", "_pos_at", "_pair_at")
+    __slots__ = ("tokens", "top_k", "rows", "e_local", "local_expert_offset", "align", "device", "_table", "_pos_at", "_pair_at", "_pointers")
 
     def __init__(self, device, tokens, top_k, rows, e_local, local_expert_offset, align):
         self.tokens, self.top_k, self.rows = tokens, top_k, rows
@@ -299,16 +299,23 @@ class TokenOrder:
         # offsets, counts, pos, pair: the latter two at multiples of 16 bytes
         self._pos_at = (2 * e_local + 4) // 4 * 4
         self._pair_at = self._pos_at + (tokens * top_k + 3) // 4 * 4
-        self._table = torch.empty(self._pair_at + rows, dtype=torch.int32, device=device)
+        self._own(torch.empty(self._pair_at + rows, dtype=torch.int32, device=device))
 
-    def _pointers(self) -> Tuple[int, int, int]:
-        """Addresses of pos, pair and offsets.  Asked of the table at every call: a copied or unpickled order has its own."""
-        ptr = self._table.data_ptr()
-        return ptr + 4 * self._pos_at, ptr + 4 * self._pair_at, ptr
+    def _own(self, table: torch.Tensor) -> None:
+        """Takes the table, and from it the device and the addresses of pos, pair and offsets."""
+        ptr = table.data_ptr()
+        self._table, self.device = table, table.device
+        self._pointers = ptr + 4 * self._pos_at, ptr + 4 * self._pair_at, ptr
 
-    @property
-    def device(self) -> torch.device:
-        return self._table.device
+    # a copied or unpickled order has a table of its own, elsewhere
+    def __getstate__(self):
+        return {name: getattr(self, name) for name in self.__slots__ if name not in ("device", "_pointers")}
+
+    def __setstate__(self, state):
+        for name, value in state.items():
+            if name != "_table":
+                setattr(self, name, value)
+        self._own(state["_table"])
 
     @property
     def offsets(self) -> torch.Tensor:
@@ -358,7 +365,7 @@ def sort_tokens(topk_ids: torch.Tensor, e_local: int = E_GLOBAL, local_expert_of
     if pairs > _SORT_ONE_LAUNCH:
         ws_bytes = _capi.lib().b200moe_sort_workspace_bytes(tokens, top_k, e_local)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    pos, pair, offsets = order._pointers()
+    pos, pair, offsets = order._pointers
     _call("b200moe_sort_tokens", dev.index, ids.data_ptr(), ids.element_size() * 8, pitch, tokens, top_k, e_local, off, align,
           offsets + 4 * (e_local + 1), offsets, pos, pair, rows, None if ws is None else ws.data_ptr(), ws_bytes)
     return order
@@ -371,8 +378,8 @@ def _permute(x: torch.Tensor, order: TokenOrder, out: Optional[torch.Tensor]) ->
         y = torch.empty(order.rows, H, dtype=x.dtype, device=x.device)
     else:
         y_pitch = _pitch(out)
-    _call("b200moe_permute_rows", x.device.index, x.data_ptr(), pitch * size, H * size, size, order.tokens, order.top_k,
-          *order._pointers(), order.e_local, order.rows, y.data_ptr(), y_pitch * size, int(out is None))
+    _call("b200moe_permute_rows", order.device.index, x.data_ptr(), pitch * size, H * size, size, order.tokens, order.top_k,
+          *order._pointers, order.e_local, order.rows, y.data_ptr(), y_pitch * size, int(out is None))
     if out is not None:
         _written(out)
     return y
@@ -389,7 +396,7 @@ def _unpermute(y: torch.Tensor, order: TokenOrder, weights: Optional[torch.Tenso
         res = torch.empty(order.tokens, H, dtype=y.dtype, device=y.device)
     else:
         res_pitch = _pitch(out)
-    _call("b200moe_unpermute_rows", y.device.index, y.data_ptr(), _DTYPE[y.dtype], pitch, order._pointers()[0], w_ptr, w_pitch,
+    _call("b200moe_unpermute_rows", order.device.index, y.data_ptr(), _DTYPE[y.dtype], pitch, order._pointers[0], w_ptr, w_pitch,
           order.tokens, order.top_k, H, res.data_ptr(), res_pitch)
     if out is not None:
         _written(out)
@@ -442,7 +449,7 @@ class _Unpermute(torch.autograd.Function):
         if weights is not None:
             weights, _, _, w_pitch = _matrix(weights, "weights")
             w_ptr = weights.data_ptr()
-        pos, pair, offsets = order._pointers()
+        pos, pair, offsets = order._pointers
         _call("b200moe_unpermute_grad", dev.index, dout.data_ptr(), _DTYPE[dtype], d_pitch, y_ptr, y_pitch, w_ptr, w_pitch, pos, pair,
               offsets, order.e_local, order.tokens, order.top_k, H, rows, None if dy is None else dy.data_ptr(), H,
               None if dw is None else dw.data_ptr())

@@ -16,7 +16,7 @@ def test_addresses_are_those_of_the_copys_own_table(how):
     order._table.copy_(torch.arange(order._table.numel(), dtype=torch.int32))
     other = COPIES[how](order)
     assert other._table.data_ptr() != order._table.data_ptr()
-    assert other._pointers() == (other.pos.data_ptr(), other.pair.data_ptr(), other.offsets.data_ptr())
+    assert other._pointers == (other.pos.data_ptr(), other.pair.data_ptr(), other.offsets.data_ptr())
     for name in ("pos", "pair", "offsets", "counts"):
         assert torch.equal(getattr(other, name), getattr(order, name))
     for name in ("tokens", "top_k", "rows", "e_local", "local_expert_offset", "align", "device"):
