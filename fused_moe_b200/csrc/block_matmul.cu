@@ -930,7 +930,7 @@ extern "C" int b200moe_block_matmul(const uint8_t* a, int64_t a_row_stride, cons
     return B200MOE_ERR_INVALID_ARGUMENT;
   const uintptr_t size = out_dtype == B200MOE_F32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(a) | (uintptr_t)a_row_stride | reinterpret_cast<uintptr_t>(b) | (uintptr_t)b_row_stride) % 16 != 0 ||
-      reinterpret_cast<uintptr_t>(out) % size != 0)
+      reinterpret_cast<uintptr_t>(out) % size != 0 || !words_aligned(a_scale, b_scale, status))
     return B200MOE_ERR_MISALIGNED;
   const long long m_tiles = ((long long)M + kTile - 1) / kTile, n_tiles = ((long long)N + kTile - 1) / kTile;
   if (too_many_tiles(M, N, m_tiles, n_tiles)) return B200MOE_ERR_UNSUPPORTED_SHAPE;

@@ -7,6 +7,12 @@
 
 namespace b200moe {
 
+// Whether tables of 4-byte numbers start where such numbers may (null ones do).
+template <typename... P>
+inline bool words_aligned(const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & 3) == 0;
+}
+
 // Records the error's text for b200moe_last_cuda_error and returns B200MOE_ERR_CUDA.
 int cuda_fail(cudaError_t e, const char* what);
 

@@ -795,7 +795,8 @@ int b200moe_sort_tokens(const void* topk_ids, int ids_bits, int64_t ids_row_stri
   const int64_t need = b200moe_sort_rows(tokens, top_k, e_local, align);
   if (rows < need || need > 0x7fffffffll) return B200MOE_ERR_UNSUPPORTED_SHAPE;
   if (rows > 0 && !pair) return B200MOE_ERR_INVALID_ARGUMENT;
-  if (reinterpret_cast<uintptr_t>(topk_ids) % (ids_bits / 8) != 0 || reinterpret_cast<uintptr_t>(workspace) % 4 != 0)
+  if (reinterpret_cast<uintptr_t>(topk_ids) % (ids_bits / 8) != 0 || reinterpret_cast<uintptr_t>(workspace) % 4 != 0 ||
+      !words_aligned(counts, offsets, pos, pair))
     return B200MOE_ERR_MISALIGNED;
   const SortPlan plan = sort_plan(tokens * top_k, rows);
   if (!plan.one_launch) {
@@ -839,7 +840,8 @@ int b200moe_permute_rows(const void* x, int64_t x_row_bytes, int64_t row_bytes, 
   if (rows == 0 || row_bytes == 0) return B200MOE_OK;
   if (!pair || !offsets || !y || y_row_bytes < row_bytes || (tokens > 0 && (!x || !pos || x_row_bytes < row_bytes)))
     return B200MOE_ERR_INVALID_ARGUMENT;
-  if ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)x_row_bytes | reinterpret_cast<uintptr_t>(y) | (uintptr_t)y_row_bytes) % elem_bytes != 0)
+  if ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)x_row_bytes | reinterpret_cast<uintptr_t>(y) | (uintptr_t)y_row_bytes) % elem_bytes != 0 ||
+      !words_aligned(pos, pair, offsets))
     return B200MOE_ERR_MISALIGNED;
   int num_sms = 0;
   if ((rc = ensure_device(&num_sms)) != B200MOE_OK) return rc;
@@ -882,7 +884,8 @@ int b200moe_unpermute_rows(const void* y, int dtype, int64_t y_row_stride, const
   if (!y || !pos || !out || y_row_stride < hidden || out_row_stride < hidden || (weights && w_row_stride < top_k))
     return B200MOE_ERR_INVALID_ARGUMENT;
   const uintptr_t size = dtype == B200MOE_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(y) % size != 0 || reinterpret_cast<uintptr_t>(out) % size != 0) return B200MOE_ERR_MISALIGNED;
+  if (reinterpret_cast<uintptr_t>(y) % size != 0 || reinterpret_cast<uintptr_t>(out) % size != 0 || !words_aligned(pos, weights))
+    return B200MOE_ERR_MISALIGNED;
   int num_sms = 0;
   if ((rc = ensure_device(&num_sms)) != B200MOE_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -907,7 +910,8 @@ int b200moe_unpermute_grad(const void* dout, int dtype, int64_t dout_row_stride,
       (dw && hidden > 0 && rows > 0 && tokens > 0 && (!y || y_row_stride < hidden)))
     return B200MOE_ERR_INVALID_ARGUMENT;
   const uintptr_t size = dtype == B200MOE_F32 ? 4 : 2;
-  if ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(dy)) % size != 0)
+  if ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(dy)) % size != 0 ||
+      !words_aligned(pos, pair, offsets, weights, dw))
     return B200MOE_ERR_MISALIGNED;
   int num_sms = 0;
   if ((rc = ensure_device(&num_sms)) != B200MOE_OK) return rc;
