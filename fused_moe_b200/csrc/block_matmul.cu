@@ -9,11 +9,12 @@
 // Two kernels: 128 x 128 tiles, one CTA on an SM with four accumulators or two with two each, the K blocks of a tile divided over a
 // cluster where tiles are few; and 256 x 256 tiles of a CTA pair (cta_group::2) where there are enough of them.
 //
-// Few rows are bound by the weights' bytes and, below some 30 MB of them, by latency: one row through 4096 x 7168 takes 9.4 us (29
-// MB, 4.5 us at the copy rate), through 7168 x 16384 24.6 us (117 MB, 17.9).  Many rows are bound by the hand-offs between tensor
-// cores and promotion: 8192 x 4096 x 7168 takes 222 us, 2.2 PFLOP/s, some 1000 cycles for a K block of a tile whose MMAs take 512.
-// An accumulator's way round - issue 200 cycles, MMAs 260 to 510, the look at the barrier 200 to 300, read-back 250 to 300, the
-// counter's way back 200 and more - is longer than the MMAs of the other one, and tensor memory has no room for a third.
+// Few rows are bound by the weights' bytes and, below some 30 MB of them, by latency: one row through 4096 x 7168 takes 9.5 us from
+// HBM (29 MB, 4.5 us at the copy rate; 8.2 us from L2), through 7168 x 16384 24.7 us (117 MB, 17.9).  Many rows are bound by the
+// hand-offs between tensor cores and promotion: 8192 x 4096 x 7168 takes 203 to 222 us in a burst (by data and clock; 254 repeated, at
+// the power limit), 2.2 to 2.4 PFLOP/s, some 1000 cycles for a K block of a pair's tile whose MMAs take 512.  An accumulator's way
+// round - issue 200 cycles, MMAs 260 to 510, the look at the barrier 200 to 300, read-back 250 to 300, the counter's way back 200 and
+// more - is longer than the MMAs of the other one, and a pair's two of 256 x 256 leave no room in tensor memory for a third.
 #include "common.cuh"
 #include "host.cuh"
 #include "kernels.cuh"

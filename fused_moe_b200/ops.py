@@ -11,8 +11,12 @@ weight format, and tokens sorted by expert and back.
     out = unpermute(expert_rows, order, weights)      # differentiable in both
 
 The layer from parts is the sequence route, sort_tokens, permute, quantize, block_matmul per expert, quantize with SwiGLU,
-block_matmul, unpermute.  All results repeat bit for bit (there are no atomics on values), every call is asynchronous on the
-current stream of its tensors' device, can be captured into a CUDA graph and allocates only its results (and the sort, above
+block_matmul, unpermute.  The step in the middle is the caller's: block_matmul takes one expert's rows, so the segments
+(``order.offsets.tolist()``) have to be read on the host, which waits for the sort and cannot be captured (``run`` is the layer
+without that).  Equal calls give equal results bit for bit (there are no atomics on values); calls of other sizes may add up in
+another order (block_matmul's parts of K, see ``b200moe_block_matmul_form``, and the threads that sum a weight's gradient), so that a token's
+last bits can differ between batch sizes.  Every call is asynchronous on the current stream of its tensors' device, can be captured
+into a CUDA graph and allocates only its results (and the sort, above
 16384 pairs, a scratch tensor) from torch's allocator.  Errors: ``TypeError`` / ``ValueError`` for arguments, ``RuntimeError``
 for tensors that are not on one CUDA device, ``MoEError`` for what the library refuses, and at the next call of any operator on the
 device after a ``block_matmul`` there gave up on a bounded wait (its result holds NaN then).  A replayed graph makes no call:
@@ -168,7 +172,8 @@ def quantize(x: torch.Tensor, *, swiglu: bool = False, scale_layout: str = "kt")
 
     ``scale = max(max|x|, 1e-12) / 448`` per block, ``code = e4m3(x / scale)``, the quotient rounded to fp32 first: bit for bit
     ``synth.quant_rows_1x128``.  ``scale_layout`` "kt" gives the scales as [ceil(K/128), T], the layer's layout, "tk" as
-    [T, ceil(K/128)].  With ``swiglu`` the input is [T, 2K] and what is quantised is ``x[:, :K] * silu(x[:, K:])`` in fp32.
+    [T, ceil(K/128)].  With ``swiglu`` the input is [T, 2K] and what is quantised is ``x[:, :K] * silu(x[:, K:])`` in fp32
+    (where ``silu`` of less than -88.7 is zero: 1 + exp(-u) is infinite).
     A block that holds an infinity or a NaN gets it as its scale, and codes as the quotient says.  Any K; not differentiable.
     """
     if not x.is_cuda:
@@ -222,7 +227,8 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     a [M, K] e4m3 (or its uint8 bits) with a_scale fp32 per 1x128, [ceil(K/128), M] (``scale_layout`` "kt") or
     [M, ceil(K/128)] ("tk"); b [N, K] e4m3 with b_scale fp32 [ceil(N/128), ceil(K/128)], the layout of an expert's weights.
     K must be a multiple of 16, M and N may be any.  Rows of ``a`` whose pitch is not a multiple of 16 bytes are copied; ``b``
-    must have unit inner stride and such a pitch.  Scales may have any strides.  ``out`` writes into a tensor of the caller's
+    must have unit inner stride and such a pitch.  Scales may have any strides and values; the product of a row's and a block's is
+    rounded to fp32 before it meets the sums.  ``out`` writes into a tensor of the caller's
     (which must not overlap the inputs).  Not differentiable: the operands are codes.
     """
     if not a.is_cuda:

@@ -270,13 +270,15 @@ B200MOE_API int b200moe_ep_combine_peers(const void* const* partial_bf16, const 
 
 /* ---- operators beside the layer (no counterparts in the reference, which has the fused layer only): the layer's
  * activation format, the dense product in the experts' weight format, and tokens sorted by expert and back for experts that
- * the fused layer does not know.  Nothing here reads a workspace of the layer; all results repeat bit for bit. ---- */
+ * the fused layer does not know.  Nothing here reads a workspace of the layer.  Equal calls give equal results bit for bit; other
+ * sizes may add up in another order (b200moe_block_matmul's parts of K, the groups of threads of b200moe_unpermute_grad's dw). ---- */
 
 /* Activations to e4m3 with one scale per 1x128 block, what b200moe_run and b200moe_block_matmul take:
  *   scale[t,b] = max(max |x[t,k]| over block b, 1e-12) / 448, codes[t,k] = e4m3(fp32(x[t,k] / scale[t,b]))
  * (round to nearest even).  A block with an infinity or a NaN gets that scale, and codes as the quotient says.
  *  x        [rows, cols] of `dtype` (fp32, bf16, fp16), `row_stride` elements; swiglu != 0: [rows, 2 cols], and
- *           x[t,k] = in[t,k] * silu(in[t,cols+k]) in fp32 (the layer's order: gate half first, silu on the second)
+ *           x[t,k] = in[t,k] * silu(in[t,cols+k]) in fp32 (the layer's order: gate half first, silu on the second, zero
+ *           below -88.7, where 1 + exp(-u) is infinite)
  *  codes    [rows, cols] bytes, `codes_row_stride` bytes
  *  scale    fp32, element (t, b) at scale[t*scale_stride_t + b*scale_stride_kb], ceil(cols/128) blocks a row.
  * Any cols; the last block may be short. */
@@ -294,7 +296,8 @@ B200MOE_API int b200moe_status_words(int32_t** words);
  * share an SM.  The order of the sums goes with S.  Negative: a status. */
 B200MOE_API int b200moe_block_matmul_form(int M, int N, int K, int64_t a_row_stride, int64_t b_row_stride, int num_sms);
 
-/* out[m,n] = sum_b a_scale[m,b] * b_scale[n/128,b] * sum_{k in block b} a[m,k] * b[n,k], accumulated in fp32, rounded once.
+/* out[m,n] = sum_b a_scale[m,b] * b_scale[n/128,b] * sum_{k in block b} a[m,k] * b[n,k], accumulated in fp32, rounded once (the
+ * product of the two scales is a number of fp32 first).
  *  a        e4m3 [M, K], b e4m3 [N, K] (the experts' weight layout); row strides in bytes, multiples of 16; bases 16-byte aligned
  *  a_scale  fp32, element (m, b) at a_scale[m*a_scale_stride_m + b*a_scale_stride_kb]
  *  b_scale  fp32, element (n/128, b) at b_scale[(n/128)*b_scale_stride_n + b*b_scale_stride_kb]
