@@ -269,9 +269,9 @@ __device__ __forceinline__ bool make_factors(const MatmulParams& p, uint32_t rin
     for (int j = 0; j < kScaleBatch; ++j) {
       const int k = min(kb + j, kb1 - 1);
 #pragma unroll
-      for (int i = 0; i < R; ++i) x[j][i] = __ldg(a[i] + k * p.as_kb);
+      for (int i = 0; i < R; ++i) x[j][i] = ld_chained(a[i] + k * p.as_kb);
 #pragma unroll
-      for (int h = 0; h < H; ++h) y[j][h] = __ldg(b[h] + k * p.bs_kb);
+      for (int h = 0; h < H; ++h) y[j][h] = ld_chained(b[h] + k * p.bs_kb);
     }
 #pragma unroll
     for (int j = 0; j < kScaleBatch; ++j) {

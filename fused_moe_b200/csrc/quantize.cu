@@ -82,7 +82,7 @@ struct Raw8 {
       constexpr int kVecs = (int)sizeof(T) / 2;
       uint4 u[kVecs];
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i) u[i] = left > 0 ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < kVecs; ++i) u[i] = left > 0 ? ld_chained(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0u, 0u, 0u, 0u);
       memcpy(v, u, sizeof(v));
     } else {
 #pragma unroll
@@ -117,7 +117,7 @@ __device__ __forceinline__ float2 div2_rn_any(float2 x, float d, float inv) {
 
 template <typename T, bool SWIGLU, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads)
-quantize_kernel(const T* __restrict__ x, long long x_stride, int rows, int cols, int kblocks, uint8_t* __restrict__ codes,
+quantize_kernel(const T* x, long long x_stride, int rows, int cols, int kblocks, uint8_t* __restrict__ codes,
                 long long codes_stride, float* __restrict__ scale, long long s_stride_t, long long s_stride_kb, int log_width) {
   constexpr int kQuantUnits = quant_units(SWIGLU), kTileBlocks = kQuantUnits * kQuantHalves;
   const int width = 1 << log_width, step = kQuantHalves >> log_width, tile_rows = kTileBlocks >> log_width;   // (step: rows of a pass)

@@ -380,7 +380,7 @@ permute_kernel(const __grid_constant__ RowMove p, int segments, int segment_vecs
     V x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (v0 + u * 32 < v_end) x[u] = __ldg(src + v0 + u * 32);
+      if (v0 + u * 32 < v_end) x[u] = ld_chained(src + v0 + u * 32);
     for (int k = 0; k < p.top_k; ++k) {
       const int row = __shfl_sync(0xffffffffu, mine, k);
       if (row < 0) continue;
@@ -422,7 +422,7 @@ template <typename P>
 __device__ __forceinline__ P load_pack(const P* p) {
   P r;
   if constexpr (sizeof(P) == 16) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 u = ld_chained(reinterpret_cast<const uint4*>(p));
     memcpy(&r, &u, 16);
   } else {
     r = *p;
@@ -450,9 +450,8 @@ constexpr int kSumBatch = 8;                     // rows of a token in flight to
 // without it (with four of them 58 us).
 template <typename T, int N, int U, int GROUP, bool AHEAD>
 __global__ void __launch_bounds__(kMoveThreads, AHEAD ? 4 : 6)
-unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restrict__ pos, const float* __restrict__ weights,
-                 long long w_stride, T* __restrict__ out, long long out_stride, int items, int top_k, int row_vecs,
-                 int segments, int segment_vecs) {
+unpermute_kernel(const T* y, long long y_stride, const int* pos, const float* weights, long long w_stride, T* __restrict__ out,
+                 long long out_stride, int items, int top_k, int row_vecs, int segments, int segment_vecs) {
   using P = Pack<T, N>;
   chain_wait();
   chain_release();
@@ -462,8 +461,8 @@ unpermute_kernel(const T* __restrict__ y, long long y_stride, const int* __restr
     const int* at = pos + (size_t)t * top_k + k0;
 #pragma unroll
     for (int j = 0; j < kSumBatch; ++j) {
-      row[j] = k0 + j < top_k ? __ldg(at + j) : -1;
-      w[j] = weights && k0 + j < top_k ? __ldg(weights + (size_t)t * w_stride + k0 + j) : 1.f;
+      row[j] = k0 + j < top_k ? ld_chained(at + j) : -1;
+      w[j] = weights && k0 + j < top_k ? ld_chained(weights + (size_t)t * w_stride + k0 + j) : 1.f;
     }
   };
   const int lane = threadIdx.x % GROUP;
