@@ -129,11 +129,12 @@ def _refuse_duals(what: str, *tensors: Optional[torch.Tensor]) -> None:
 def _matrix(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
     """(``t``, rows, columns, row stride in elements) with unit inner stride, rows that do not overlap and values as they are stored (a
     copy where ``t`` has not: ``z.conj().imag`` is stored with the other sign); extents that 32 bits hold.  The stride of a single row is free: torch may say anything."""
-    if t.dim() != 2:
-        raise ValueError(f"{what} must be 2-D, got shape {tuple(t.shape)}")
-    rows, cols = t.shape
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{what} must be 2-D, got shape {tuple(shape)}")
+    rows, cols = shape
     if rows > _INT_MAX or cols > _INT_MAX:
-        raise ValueError(f"{what} must have at most {_INT_MAX} rows and columns, got shape {tuple(t.shape)}")
+        raise ValueError(f"{what} must have at most {_INT_MAX} rows and columns, got shape {tuple(shape)}")
     if t.is_neg():
         t = t.resolve_neg()
     if t.is_contiguous():
@@ -243,9 +244,10 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     if a.dtype not in _CODES or b.dtype not in _CODES:
         raise TypeError(f"a and b must be float8_e4m3fn (or its uint8 bit pattern), got {a.dtype} and {b.dtype}")
     a, M, K, a_pitch = _matrix(a, "a")
-    if b.dim() != 2 or b.shape[1] != K:
-        raise ValueError(f"b must be [N, {K}], got {tuple(b.shape)}")
-    N = b.shape[0]
+    b_shape = b.shape
+    if len(b_shape) != 2 or b_shape[1] != K:
+        raise ValueError(f"b must be [N, {K}], got {tuple(b_shape)}")
+    N = b_shape[0]
     if N > _INT_MAX:
         raise ValueError(f"b must have at most {_INT_MAX} rows, got {N}")
     if K == 0 or K % 16:
@@ -258,8 +260,10 @@ def block_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
     as_m, as_kb = _block_scale_strides(a_scale, M, blocks, scale_layout, "a_scale")
     bs_n, bs_kb = _block_scale_strides(b_scale, -(-N // BLOCK), blocks, "tk", "b_scale")
     a_ptr, b_ptr = a.data_ptr(), b.data_ptr()
-    b_pitch = K if N == 1 or b.is_contiguous() else b.stride(0)
-    if (b_ptr | b_pitch) % 16 or b_pitch < K or b.stride(1) != 1:
+    b_pitch, b_step = (K, 1) if b.is_contiguous() else b.stride()
+    if N == 1:
+        b_pitch = K
+    if (b_ptr | b_pitch) % 16 or b_pitch < K or b_step != 1:
         raise ValueError("b must have unit inner stride and rows on 16-byte boundaries")
     if (a_ptr | a_pitch) % 16:
         a = a.clone(memory_format=torch.contiguous_format)
